@@ -108,18 +108,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const char* head_bas
                            (uint32_t)max(p_end - p0, 0) * row_bytes);
 }
 
-// Lane terms of load_tile's offsets. K instruction j covers rows 2j, 2j+1 (lane i fetches the
-// chunk that belongs in LDS slot 64j + i): row r = 2j + (i>>5), chunk (i&31) ^ (r&15), i.e. byte
-// 1024j + (kl ^ 32(j&7)) with kl = 512(i>>5) + 16((i&31) ^ (i>>5)) (the swizzle moves bits 5-7
-// only). V register e, h: row 16(e>>2) + 4g4 + (e&3), dims 128h + 8c: byte
-// vl + 8192(e>>2) + 512(e&3) + 256h with vl = 2048g4 + 16c.
-struct TileLanes {
-  uint32_t kl, vl;
-  __device__ __forceinline__ explicit TileLanes(int lane)
-      : kl(512u * (lane >> 5) + 16u * ((lane & 31) ^ (lane >> 5))),
-        vl(2048u * (lane >> 4) + 16u * (lane & 15)) {}
-};
-
 // Issue one tile's loads: 16 LDS-DMA loads of K (each reads 1 KB of contiguous cache into the
 // wave's K tile at LDS byte ks_s), then 16 register loads of V (4 rows x 256 B per instruction).
 // krs / vrs are the tile's resources (tile_rsrc). The scheduling barrier keeps every K load ahead
@@ -158,13 +146,6 @@ __device__ __forceinline__ void issue_v(VTile& b, __amdgpu_buffer_rsrc_t vrs, co
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       b.v[e][h] = buffer_load16_stream(vrs, vl + 8192u * (e >> 2) + 512u * (e & 3) + 256u * h);
-}
-
-// Order this wave's LDS accesses: the compiler must not move LDS reads/writes across it (lanes
-// exchange data through LDS, which single-thread alias analysis cannot see).
-__device__ __forceinline__ void wave_lds_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
 }
 
 // Compute one tile whose K has landed in the wave's LDS slot ks_lds and whose V registers are
@@ -272,42 +253,6 @@ __device__ __forceinline__ void fused_place_tile(KRegs& kr, VTile& b, u32x4_t* k
 struct VTile8 {
   u32x2_t v[8][2];  // V rows P(g4, e), dims 128h + 8c + [0, 8), as fp8 codes
 };
-
-// Lane terms of the fp8 tile loads' offsets (tile resources as for bf16). K instruction j: row
-// r = 4j + (i>>4), chunk (i&15) ^ (r&15), i.e. byte 1024j + (kl ^ 64(j&3)) with
-// kl = 256(i>>4) + 16((i&15) ^ (i>>4)). V register e, h: byte vl + 4096(e>>2) + 256(e&3) + 128h
-// with vl = 1024g4 + 8c.
-struct TileLanes8 {
-  uint32_t kl, vl;
-  __device__ __forceinline__ explicit TileLanes8(int lane)
-      : kl(256u * (lane >> 4) + 16u * ((lane & 15) ^ (lane >> 4))),
-        vl(1024u * (lane >> 4) + 8u * (lane & 15)) {}
-};
-
-// S^T = K Q^T from an fp8 K tile in LDS: lane (c, g4) reads the 8 codes of row 16T + c, dims
-// [32ks + 8g4, +8) (half of the swizzled 16-byte chunk 2ks + g4/2) and converts them to the bf16
-// A operand of qk_tile. With the tile 256-byte aligned, chunk (2ks + g4/2) ^ c at byte 16 chunk
-// is one per-lane base XORed with 32 ks (the swizzle moves bits 5-7 only) plus 4096 T.
-template <int NT>
-__device__ __forceinline__ void qk_tile8(const u32x4_t* k_lds, const bf16x8_t (&qb)[NT][8], int c,
-                                         int g4, f32x4_t (&sacc)[NT][2]) {
-  typedef __attribute__((address_space(3))) const u32x2_t lds_u32x2;
-  const uint32_t b0 =
-      (uint32_t)(uintptr_t)((__attribute__((address_space(3))) const char*)reinterpret_cast<const char*>(k_lds)) +
-      c * 256 + 16 * (c & 14) + 16 * ((g4 >> 1) ^ (c & 1)) + 8 * (g4 & 1);
-#pragma unroll
-  for (int T = 0; T < 2; ++T) {
-#pragma unroll
-    for (int ct = 0; ct < NT; ++ct) sacc[ct][T] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      const u32x2_t w = *(lds_u32x2*)(uintptr_t)((b0 ^ (32u * ks)) + 4096 * T);
-      const bf16x8_t kop = as_bf16x8(fp8x8_to_bf16x8(w));
-#pragma unroll
-      for (int ct = 0; ct < NT; ++ct) sacc[ct][T] = mfma16x16x32(kop, qb[ct][ks], sacc[ct][T]);
-    }
-  }
-}
 
 // One fp8 tile's loads for the look-ahead loop: the K codes (8 KB) into one of the wave's two LDS
 // K slots (8 LDS-DMA loads), and the V codes into registers (16 loads of 8 bytes).
