@@ -28,6 +28,8 @@ from ._C import (  # noqa: E402,F401
     attn_decode_combine,
     attn_decode_fp8,
     attn_decode_fp8_partials,
+    attn_decode_paged,
+    attn_decode_paged_fp8,
     attn_decode_partials,
     attn_prefill,
     attn_prefill_ws,
@@ -35,10 +37,17 @@ from ._C import (  # noqa: E402,F401
     attn_prep_chunk,
     attn_prep_decode,
     attn_prep_fp8,
+    attn_prep_paged,
+    attn_prep_paged_fp8,
     commit,
     embed,
     gdn_step_n,
     gemv_bf16,
+    kv_pages_compact,
+    kv_pages_copy,
+    kv_pages_extend,
+    kv_pages_fork,
+    kv_pages_free,
     l2_persist_limit,
     mtp_select,
     prefill_ws_bytes,

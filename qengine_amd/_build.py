@@ -1,7 +1,7 @@
 """Build recipe for qengine_amd's native code (no setuptools, no hipify).
 
   libqe_attn.so  : gfx950 HIP kernels + the C ABI of include/qe_attn.h, include/qe_gemv.h,
-                   include/qe_step.h and include/qe_gdn.h (hipcc).
+                   include/qe_step.h, include/qe_gdn.h and include/qe_paged.h (hipcc).
   _C<ext>.so     : torch extension with the reference's op signatures (g++ against torch's
                    ROCm build), linked to libqe_attn.so through $ORIGIN.
 
@@ -26,7 +26,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
 HIP_SOURCES = ["attn_prep.hip", "attn_decode.hip", "attn_combine.hip", "attn_prefill.hip",
-               "attn_prefill_wide.hip",
+               "attn_prefill_wide.hip", "attn_paged.hip", "attn_prep_paged.hip", "kv_pages.hip",
                "gemv.hip", "gemv_lds.hip", "step.hip", "gdn.hip", "gdn_split.hip"]
 # Per-source code-generation flags. The prefill tile loop keeps 128 fp32 accumulators live; the
 # compiler's default MFMA register form parks them in AGPRs and copies all of them into VGPRs
@@ -40,6 +40,7 @@ MAX_ILP = ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]
 SOURCE_FLAGS = {"attn_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", *MAX_ILP],
                 "attn_prefill_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", *MAX_ILP],
                 "attn_combine.hip": MAX_ILP, "gdn_split.hip": MAX_ILP, "gemv_lds.hip": MAX_ILP}
+BINDINGS = ["bindings", "bindings_paged"]  # .cpp
 LIB = PKG / "libqe_attn.so"
 EXT = PKG / ("_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 
@@ -87,14 +88,21 @@ def build_ext() -> Path:
     tlib = Path(torch.__file__).resolve().parent / "lib"
     incs = [*ce.include_paths(device_type="cuda"), sysconfig.get_paths()["include"], str(INCLUDE)]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    obj = OBJ / "bindings.o"
     OBJ.mkdir(exist_ok=True)
-    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-variable",
-          "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_C",
-          "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-          *[f"-I{i}" for i in incs], "-c", str(CSRC / "bindings.cpp"), "-o", str(obj)])
+
+    def compile_one(name: str) -> str:
+        obj = OBJ / (name + ".o")
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-variable",
+              "-Wno-unused-function", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+              "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
+              f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *[f"-I{i}" for i in incs], "-c",
+              str(CSRC / (name + ".cpp")), "-o", str(obj)])
+        return str(obj)
+
+    with ThreadPoolExecutor(max_workers=2) as ex:
+        objs = list(ex.map(compile_one, BINDINGS))
     tmp = EXT.with_suffix(".tmp")
-    _run(["g++", "-shared", "-fPIC", str(obj), "-o", str(tmp),
+    _run(["g++", "-shared", "-fPIC", *objs, "-o", str(tmp),
           f"-L{PKG}", "-lqe_attn", f"-L{tlib}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
           "-ltorch_hip", "-ltorch_python", "-lamdhip64",
           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"])

@@ -1,5 +1,5 @@
-"""ctypes binding of the C ABI in include/qe_attn.h, include/qe_gemv.h, include/qe_step.h and
-include/qe_gdn.h (libqe_attn.so), without the torch extension.
+"""ctypes binding of the C ABI in include/qe_attn.h, include/qe_gemv.h, include/qe_step.h,
+include/qe_gdn.h and include/qe_paged.h (libqe_attn.so), without the torch extension.
 
 This is the binding a non-torch host (or a test that must go through the C ABI) uses. Tensor
 arguments may be torch tensors (their data_ptr is passed) or raw integer device addresses.
@@ -62,6 +62,17 @@ SIGNATURES = {
     "qe_mtp_select": (_I, [_P, _P, _I, _P, _L, _P, _I, _P, _P, _P]),
     "qe_l2_persist_limit": (_I, [ctypes.c_size_t]),
     "qe_stream_access_window": (_I, [ctypes.c_size_t, ctypes.c_size_t, _F, _P]),
+    "qe_attn_decode_paged": (_I, [_P, _P, _P, _P, _L, _P, _P, _L, _P, _P, _P, _L] + [_I] * 10 + [_F, _P]),
+    "qe_attn_decode_paged_fp8": (_I, [_P, _P, _P, _P, _L, _P, _P, _L, _P, _P, _P, _L] + [_I] * 10
+                                 + [_F, _F, _F, _P]),
+    "qe_attn_prep_paged": (_I, [_P, _P, _P, _L] + [_P] * 8 + [_L] + [_I] * 8 + [_F, _P]),
+    "qe_attn_prep_paged_fp8": (_I, [_P, _P, _P, _L] + [_P] * 8 + [_L] + [_I] * 8 + [_F, _F, _F, _P]),
+    "qe_kv_pages_free": (_I, [_P, _L, _P, _P, _P, _I, _I, _I, _I, _P]),
+    "qe_kv_pages_extend": (_I, [_P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
+    "qe_kv_pages_ws_size": (_Z, [_I]),
+    "qe_kv_pages_fork": (_I, [_P, _L, _P, _P, _P, _P, _I, _P, _P, _I, _Z, _P, _P, _I, _I, _I, _I, _P]),
+    "qe_kv_pages_compact": (_I, [_P, _L, _P, _P, _P, _I, _Z, _P, _I, _I, _I, _P]),
+    "qe_kv_pages_copy": (_I, [_P, _P, _I, _Z, _P, _P, _I, _I, _P]),
     "qe_gdn_step_n": (_I, [_P, _P, _P, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I,
                            _I, _F, _P]),
 }

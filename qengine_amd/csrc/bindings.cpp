@@ -12,72 +12,13 @@
 //
 // The _check_* functions run the same validation without the device requirement and without a
 // launch, so the contract can be exercised on a machine without a GPU.
-#include <cmath>
-#include <limits>
-
-#include <torch/extension.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-
 #include "qe_attn.h"
 #include "qe_gdn.h"
 #include "qe_gemv.h"
 #include "qe_step.h"
+#include "bindings_util.hpp"
 
 namespace {
-const auto BF = torch::kBFloat16;
-const auto I32 = torch::kInt32;
-const auto F32 = torch::kFloat32;
-constexpr int HD = 256;
-
-hipStream_t stream_of(const torch::Tensor& t) {
-  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
-}
-
-void chk(const torch::Tensor& t, torch::ScalarType dt, const char* name, bool dev) {
-  if (dev) TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
-  TORCH_CHECK(t.scalar_type() == dt, name, " has wrong dtype ", t.scalar_type());
-  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
-}
-
-// Row view: (rows, width, row stride).
-struct Rows {
-  int n;
-  long w;
-  long ld;
-};
-Rows rows(const torch::Tensor& t, torch::ScalarType dt, const char* name, bool dev) {
-  TORCH_CHECK((!dev || t.is_cuda()) && t.scalar_type() == dt, name, ": wrong device/dtype");
-  if (t.dim() == 1) {
-    TORCH_CHECK(t.stride(0) == 1, name, " not contiguous");
-    return {1, (long)t.size(0), (long)t.size(0)};
-  }
-  TORCH_CHECK(t.dim() == 2 && t.stride(1) == 1, name, " must be [n, w] with unit inner stride");
-  return {(int)t.size(0), (long)t.size(1), (long)t.stride(0)};
-}
-
-void chk16(const torch::Tensor& t, long ld, const char* name) {
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && ld % 8 == 0, name,
-              " must be 16-byte aligned rows");
-}
-
-// The fp8 KV cache: E4M3FN codes, as torch.float8_e4m3fn or raw uint8 bytes.
-void chk_kv8(const torch::Tensor& t, const char* name, bool dev) {
-  if (dev) TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
-  TORCH_CHECK(t.scalar_type() == torch::kFloat8_e4m3fn || t.scalar_type() == torch::kByte, name,
-              " must be float8_e4m3fn (or uint8 codes), got ", t.scalar_type());
-  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
-}
-
-void chk_pos(const torch::Tensor& pos, bool dev) {
-  TORCH_CHECK((!dev || pos.is_cuda()) && pos.scalar_type() == I32 && pos.numel() >= 1,
-              "pos must be an int32 GPU tensor with at least one element");
-}
-
-void raise_on(hipError_t e, const char* what) {
-  TORCH_CHECK(e == hipSuccess, what, " failed: ", hipGetErrorString(e));
-}
-
 struct PrepArgs {
   int n, Hq, Hkv, max_len, rd;
   long ldp;
@@ -368,16 +309,6 @@ std::vector<int64_t> check_attn_decode(torch::Tensor q, torch::Tensor kc, torch:
 // ---- fp8 KV cache (no reference counterpart: the reference cache is bf16, engine.py:419) ------
 // attn_prep / attn_decode over a cache of E4M3FN codes with per-cache scales: a stored code c
 // means c * scale; prep stores round-to-nearest-even(x / scale), saturated at +-448.
-void kv_scales(double k_scale, double v_scale) {
-  // as fp32, the kernels' type: normal and finite, so that 1/scale is finite too
-  const auto ok = [](double s) {
-    const float f = (float)s;
-    return f >= std::numeric_limits<float>::min() && f <= std::numeric_limits<float>::max();
-  };
-  TORCH_CHECK(ok(k_scale) && ok(v_scale),
-              "k_scale and v_scale must be positive, finite and not subnormal as fp32");
-}
-
 void attn_prep_fp8(torch::Tensor qg, torch::Tensor k, torch::Tensor v, torch::Tensor qnw,
                    torch::Tensor knw, torch::Tensor inv_freq, torch::Tensor pos, torch::Tensor q_out,
                    torch::Tensor kc8, torch::Tensor vc8, double eps, double k_scale,
@@ -717,6 +648,8 @@ void gdn_step_n(torch::Tensor qkv, torch::Tensor z, torch::Tensor b, torch::Tens
            "qe_gdn_step_n");
 }
 
+void bind_paged(py::module_& m);  // bindings_paged.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "MI355X (gfx950) gated-attention decode ops with qengine._C's signatures";
   m.def("attn_prep", &attn_prep);
@@ -840,4 +773,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "no-op: the reference's phase-parallel A/B switch (one code path here)");
   m.def("set_gdn_early", [](bool) {},
         "no-op: the reference's overlap-with-producer A/B switch (no dependent launch on HIP)");
+  bind_paged(m);
 }
