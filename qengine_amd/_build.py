@@ -39,6 +39,7 @@ HIP_SOURCES = ["attn_prep.hip", "attn_decode.hip", "attn_combine.hip", "attn_pre
 MAX_ILP = ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]
 SOURCE_FLAGS = {"attn_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", *MAX_ILP],
                 "attn_prefill_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", *MAX_ILP],
+                "attn_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                 "attn_combine.hip": MAX_ILP, "gdn_split.hip": MAX_ILP, "gemv_lds.hip": MAX_ILP}
 BINDINGS = ["bindings", "bindings_paged"]  # .cpp
 LIB = PKG / "libqe_attn.so"

@@ -5,10 +5,9 @@
 // of 32-position tiles, S^T = K Q^T and O^T += V^T P^T on MFMA, K one tile ahead through LDS DMA, V in
 // registers. What differs:
 //  * A tile is two halves of 16 positions with a buffer resource each, whose base comes from the page
-//    table; a lane holds the page of one of the wave's next 64 tiles and readlane hands it out, so the
-//    loop waits for no table entry. Pages are powers of two >= 16, so no half crosses a page.
-//  * The grid is a list of (sequence, slice, KV head) items that every workgroup derives from pos: a wave
-//    scan over the sequences' slice counts. Work goes by the lengths at hand, not by the longest possible.
+//    table, read a tile ahead. Pages are powers of two >= 16, so no half crosses a page.
+//  * Persistent workgroups take equal parts of the call's work, which each derives from pos: a wave scan over
+//    the sequences' tiles. Work goes by the lengths at hand, not by the longest possible.
 //  * Slices start at multiples of their size and tiles go to waves by their place in the slice, both
 //    counted from position 0. So the rows of a call share a slice whatever their windows, a tile that a
 //    row does not attend is an exact no-op for it, and a row's bits depend on no other row or sequence.
@@ -18,6 +17,7 @@
 //  * The output is rounded once: bf16(O / L * sigmoid(gate)) in fp32 (the contiguous decode keeps the
 //    rounding points of the reference, which has no paged cache).
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_split.hpp"
 #include "attn_tile.hpp"
@@ -37,14 +37,20 @@ struct Call {
   NsDiv nd;
   int window, sinks;
   int rc, hc, hch;                   // rows and heads of a column chunk, head chunks
+  int parts;                         // workgroups of a KV head
   uint32_t hkv_m;                    // floor(2^32 / Hkv), or 2^32 - 1
   long ldt, ldp, ldo;
   float scale_log2, v_scale;
 };
 
-// ceil(x / d), floor(x / d) for 0 <= x < 2^24, 0 < d: the quotient, correctly rounded to 24 bits, is below
-// the next whole number where the exact one is (it is by at least 1 / d > x / d * 2^-24).
-__device__ __forceinline__ int div_floor(int x, int d) { return (int)((float)x / (float)d); }
+// floor(x / d), ceil(x / d) for 0 <= x < 2^24, d >= 32: the estimate is off by less than one (the reciprocal
+// and the product by 2^-22 of x / d < 2^19), then corrected.
+__device__ __forceinline__ int div_floor(int x, int d) {
+  int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
+  const int r = x - q * d;
+  q += r >= d;
+  return q - (r < 0);
+}
 __device__ __forceinline__ int div_ceil(int x, int d) { return div_floor(x + d - 1, d); }
 
 // Slices of the row at position p: size ch, slice i is [i ch, (i + 1) ch). Those of a row without a gap
@@ -59,15 +65,27 @@ __device__ __forceinline__ int count_to(const RowSlices& s, int L) {  // slices 
   const int nch = div_ceil(L, s.ch);
   return s.gap ? s.nsk + (s.lo < L ? max(nch - s.wlo, 0) : 0) : nch;
 }
+// split_size, above 128 positions (a tile for every wave) in multiples of 128
+__device__ __forceinline__ int slice_size(const Call& a, int L) {
+  constexpr int ALL = WAVES * TILE;
+  const int ch = split_size(L, a.nd);
+  return max(a.mins, ch <= ALL ? ch : (ch + ALL - 1) / ALL * ALL);
+}
 __device__ __forceinline__ RowSlices row_slices(const Call& a, int p) {
   RowSlices s;
   s.L = min(p + 1, a.cap);
-  s.lo = a.window ? max(p + 1 - a.window, 0) : 0;
-  s.gap = s.lo > a.sinks;
-  const int V = a.window ? min(s.L, a.sinks + a.window) : s.L;
-  s.ch = max(a.mins, split_size(V, a.nd));
-  s.nsk = s.gap ? div_ceil(a.sinks, s.ch) : 0;
-  s.wlo = s.gap ? max(div_floor(min(s.lo, a.cap), s.ch), s.nsk) : 0;
+  s.lo = s.nsk = s.wlo = 0, s.gap = false;
+  if (a.window) {
+    s.lo = max(p + 1 - a.window, 0);
+    s.gap = s.lo > a.sinks;
+    s.ch = slice_size(a, min(s.L, a.sinks + a.window));
+    if (s.gap) {
+      s.nsk = div_ceil(a.sinks, s.ch);
+      s.wlo = max(div_floor(min(s.lo, a.cap), s.ch), s.nsk);
+    }
+  } else {
+    s.ch = slice_size(a, s.L);
+  }
   s.cnt = count_to(s, s.L);
   return s;
 }
@@ -78,23 +96,28 @@ __device__ __forceinline__ int slot_of(const RowSlices& s, int i) {
   return i >= s.wlo && k < s.cnt ? k : -1;
 }
 
-// The slices of a sequence's rows [tc, tc + rn): rows [0, tB) have one size, rows [tB, rn) the next (the
-// size is a step function of the length with steps of 32 NS positions or more, and rn <= 8). pos >= 0.
+// The items of a sequence's rows at positions p0 .. p0 + rn - 1 (p0 >= 0): the slices of rows [0, tB), which
+// have one size, then those of rows [tB, rn), which have the next (the size is a step function of the length
+// with steps of 32 NS positions or more, and rn <= 8).
 struct SeqItems {
-  int tB, nA, nB;
+  RowSlices f;  // of the first row
+  int tB, nA, n;
 };
 __device__ __forceinline__ SeqItems seq_items(const Call& a, int p0, int rn) {
-  const RowSlices f = row_slices(a, p0);
-  SeqItems q{rn, 0, 0};
-  const RowSlices l = row_slices(a, p0 + rn - 1);
-  if (f.ch == l.ch) {
-    q.nA = count_to(f, l.L);
-  } else {
-    int t = 1;
-    while (row_slices(a, p0 + t).ch == f.ch) ++t;
-    q.tB = t;
-    q.nA = count_to(f, min(p0 + t, a.cap));
-    q.nB = count_to(row_slices(a, p0 + t), l.L);
+  SeqItems q;
+  q.f = row_slices(a, p0);
+  q.tB = rn, q.nA = q.n = q.f.cnt;
+  if (rn > 1) {
+    const RowSlices l = row_slices(a, p0 + rn - 1);
+    if (q.f.ch == l.ch) {
+      q.nA = q.n = count_to(q.f, l.L);
+    } else {
+      int t = 1;
+      while (row_slices(a, p0 + t).ch == q.f.ch) ++t;
+      q.tB = t;
+      q.nA = count_to(q.f, min(p0 + t, a.cap));
+      q.n = q.nA + count_to(row_slices(a, p0 + t), l.L);
+    }
   }
   return q;
 }
@@ -112,57 +135,111 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// One item: rows [r0, r1) of the chunk, slice [beg, end) of sequence b.
+// One item: rows [r0, r1) of the chunk (whose first row is at position p0), slice [beg, end) of sequence b.
 struct Item {
-  int b, p0;  // position of the chunk's first row
-  int r0, r1, slice, beg, end;
+  int b, p0, r0, r1, slice, beg, end;
 };
 
-// The x-th item of the call's chunk of rows [tc, tc + rn); false past the last one. Uniform.
-__device__ __forceinline__ bool find_item(const Call& a, const int* pos, int tc, int rn, int x, int lane,
-                                          Item& it) {
-  const int K = (a.B + WAVE - 1) / WAVE;  // sequences per lane, consecutive
-  int mine = 0, p = -1;
-  for (int i = 0; i < K; ++i) {
-    const int b = lane * K + i;
-    p = b < a.B ? pos_of(pos, b) : -1;
-    if (p >= 0) {
-      const SeqItems q = seq_items(a, p + tc, rn);
-      mine += q.nA + q.nB;
-    }
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Where a workgroup is in a sequence's items (SeqItems, in scalar registers).
+struct Cursor {
+  Item it;
+  int k, nA, n, tB;      // the item's number
+  int ch, nsk, wlo, lo;  // the first row's slices
+  int at, len, hi;       // (parts of a line, below)
+};
+__device__ __forceinline__ SeqItems open_sequence(const Call& a, Cursor& c, int b, int p, int tc, int rn) {
+  c.it.b = b, c.it.p0 = p + tc;
+  const SeqItems q = seq_items(a, c.it.p0, rn);
+  c.k = 0, c.nA = uni(q.nA), c.n = uni(q.n), c.tB = uni(q.tB);
+  c.ch = uni(q.f.ch), c.nsk = uni(q.f.nsk), c.wlo = uni(q.f.wlo), c.lo = uni(q.f.lo);
+  return q;
+}
+__device__ __forceinline__ void place_item(const Call& a, int rn, Cursor& c) {
+  int k = c.k, nsk = c.nsk, wlo = c.wlo, ch = c.ch;
+  c.it.r0 = 0, c.it.r1 = c.tB;
+  if (k >= c.nA) {
+    const RowSlices s = row_slices(a, c.it.p0 + c.tB);
+    k -= c.nA, nsk = uni(s.nsk), wlo = uni(s.wlo), ch = uni(s.ch);
+    c.it.r0 = c.tB, c.it.r1 = rn;
   }
-  const int upto = wave_scan(mine);
-  const int at = __popcll(__ballot(upto <= x));  // the lane whose sequences hold item x
-  if (at >= WAVE) return false;
-  x -= __builtin_amdgcn_readlane(upto - mine, at);
-  SeqItems q;
-  for (int i = 0;; ++i) {
-    if (i >= K) return false;  // (pos changed meanwhile)
-    it.b = at * K + i;
-    p = K == 1 ? __builtin_amdgcn_readlane(p, at) : __builtin_amdgcn_readfirstlane(pos_of(pos, it.b));
-    if (p >= 0) {
-      q = seq_items(a, p + tc, rn);
-      q.nA = __builtin_amdgcn_readfirstlane(q.nA);
-      q.nB = __builtin_amdgcn_readfirstlane(q.nB);
-      if (x < q.nA + q.nB) break;
-      x -= q.nA + q.nB;
-    }
-  }
-  it.p0 = p + tc;
-  const bool second = x >= q.nA;
-  it.r0 = second ? q.tB : 0;
-  it.r1 = second ? rn : q.tB;
-  const int k = second ? x - q.nA : x;
-  const RowSlices s = row_slices(a, it.p0 + it.r0);
-  it.slice = __builtin_amdgcn_readfirstlane(k < s.nsk ? k : k - s.nsk + s.wlo);
-  const int ch = __builtin_amdgcn_readfirstlane(s.ch);
-  it.beg = it.slice * ch;
-  it.end = min(it.beg + ch, min(it.p0 + it.r1, a.cap));
-  return true;
+  c.it.slice = k < nsk ? k : k - nsk + wlo;
+  c.it.beg = c.it.slice * ch;
+  c.it.end = min(c.it.beg + ch, min(c.it.p0 + c.it.r1, a.cap));
 }
 
-// ---- a tile of the paged cache: two halves of 16 positions, a resource each
-struct Halves {
+// The items of a batch: a sequence's lie along a line, one after another, each as long as its tiles plus
+// OVER, and the sequences follow one another. Workgroup i of a KV head takes the items that begin in the i-th
+// of equal parts of the line. Places count from the part's begin.
+constexpr int OVER = 3;  // what an item costs beside its tiles, in tiles
+
+// A sequence's length on the line: a little more than its tiles, and OVER for each item.
+__device__ __forceinline__ int line_of(const Call& a, const SeqItems& q, int p0, int rn) {
+  const int last = min(p0 + rn, a.cap);
+  const int tiles = q.f.gap ? max(last - q.f.lo, 0) / TILE + a.sinks / TILE + 2 : (last + TILE - 1) / TILE;
+  return q.n * OVER + tiles;
+}
+__device__ __forceinline__ int place_of(const Call& a, const Cursor& c) {
+  const int tiles = c.k < c.nsk || c.nsk + c.wlo == 0
+                        ? c.k * c.ch / TILE
+                        : a.sinks / TILE + 1 + max((c.wlo + c.k - c.nsk) * c.ch - c.lo, 0) / TILE;
+  return c.at + min(c.k * OVER + tiles, c.len - 1);
+}
+__device__ __forceinline__ void open_on_line(const Call& a, Cursor& c, int b, int p, int tc, int rn) {
+  const SeqItems q = open_sequence(a, c, b, p, tc, rn);
+  c.len = uni(line_of(a, q, c.it.p0, rn));
+}
+// The cursor's item, if it begins in the part. At the end of a sequence: the next one's first.
+__device__ __forceinline__ bool take_item(const Call& a, const int* pos, int tc, int rn, Cursor& c) {
+  while (c.k >= c.n) {
+    c.at += c.len;
+    int b = c.it.b, p = -1;
+    while (p < 0) {
+      if (++b >= a.B) return false;
+      p = pos_of(pos, uni(b));
+    }
+    open_on_line(a, c, b, p, tc, rn);
+  }
+  if (place_of(a, c) >= c.hi) return false;
+  place_item(a, rn, c);
+  return true;
+}
+// The first item of part i of `parts`.
+__device__ __forceinline__ bool first_item(const Call& a, const int* pos, int tc, int rn, int i, int parts,
+                                           int lane, Cursor& c) {
+  const int K = (a.B + WAVE - 1) / WAVE;  // sequences per lane, consecutive
+  int mine = 0, p = -1;
+  for (int s = 0; s < K; ++s) {
+    const int b = lane * K + s;
+    p = b < a.B ? pos_of(pos, b) : -1;
+    if (p >= 0) mine += line_of(a, seq_items(a, p + tc, rn), p + tc, rn);
+  }
+  const int upto = wave_scan(mine);
+  const int total = __builtin_amdgcn_readlane(upto, WAVE - 1);
+  const int part = uni((int)(((unsigned)total + parts - 1) / (unsigned)parts)), lo = i * part;
+  c.hi = min(part, total - lo);
+  const int at = __popcll(__ballot(upto <= lo));  // the lane whose sequences hold the part's begin
+  if (lo >= total || at >= WAVE) return false;
+  c.at = __builtin_amdgcn_readlane(upto - mine, at) - lo;
+  for (int s = 0;; ++s) {
+    const int b = at * K + s;
+    if (s >= K || b >= a.B) return false;  // (pos changed meanwhile)
+    const int q = K == 1 ? __builtin_amdgcn_readlane(p, at) : uni(pos_of(pos, b));
+    if (q < 0) continue;
+    open_on_line(a, c, b, q, tc, rn);
+    if (c.at + c.len > 0) break;
+    c.at += c.len;
+  }
+  // the first item from the part's begin on: an estimate, then steps
+  c.k = min(max(-c.at, 0) / (c.ch / TILE + OVER), c.n);
+  while (c.k > 0 && (c.k >= c.n || place_of(a, c) >= 0)) --c.k;
+  while (c.k < c.n && place_of(a, c) < 0) ++c.k;
+  return take_item(a, pos, tc, rn, c);
+}
+
+// ---- a tile of the paged cache: one buffer resource, or with pages of 16 positions (P16) one for each half
+struct Rsrc {
   __amdgpu_buffer_rsrc_t h[2];
 };
 template <bool KV8>
@@ -174,30 +251,27 @@ struct Tile<true> {
   u32x2_t v[8][2];
 };
 
-template <bool KV8>
-__device__ __forceinline__ void issue_k(uint32_t ks_s, const Halves& r, uint32_t kl) {
+template <bool KV8, bool P16>
+__device__ __forceinline__ void issue_k(uint32_t ks_s, const Rsrc& r, uint32_t kl) {
   asm volatile("" : "+v"(kl));  // offsets formed at each issue, not kept across the loop
-  if constexpr (KV8) {
+  constexpr int N = KV8 ? 8 : 16, HALF = P16 ? N / 2 : N, SWZ = KV8 ? 64 : 32, CYC = KV8 ? 4 : 8;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      buffer_load16_to_lds_at(r.h[j >> 2], (kl ^ (64u * (j & 3))) + 1024u * (j & 3), ks_s + 1024u * j);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      buffer_load16_to_lds_at(r.h[j >> 3], (kl ^ (32u * (j & 7))) + 1024u * (j & 7), ks_s + 1024u * j);
-  }
+  for (int j = 0; j < N; ++j)
+    buffer_load16_to_lds_at(r.h[j / HALF], (kl ^ (SWZ * (j % CYC))) + 1024u * (j % HALF), ks_s + 1024u * j);
 }
-template <bool KV8>
-__device__ __forceinline__ void issue_v(Tile<KV8>& t, const Halves& r, uint32_t vl) {
+template <bool KV8, bool P16>
+__device__ __forceinline__ void issue_v(Tile<KV8>& t, const Rsrc& r, uint32_t vl) {
   asm volatile("" : "+v"(vl));
+  constexpr uint32_t ROW = KV8 ? 256 : 512;
 #pragma unroll
   for (int e = 0; e < 8; ++e)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      const uint32_t off = vl + ROW * (e & 3) + ROW / 2 * h + (P16 ? 0 : 16 * ROW * (e >> 2));
       if constexpr (KV8)
-        t.v[e][h] = buffer_load8_stream(r.h[e >> 2], vl + 256u * (e & 3) + 128u * h);
+        t.v[e][h] = buffer_load8_stream(r.h[P16 ? e >> 2 : 0], off);
       else
-        t.v[e][h] = buffer_load16_stream(r.h[e >> 2], vl + 512u * (e & 3) + 256u * h);
+        t.v[e][h] = buffer_load16_stream(r.h[P16 ? e >> 2 : 0], off);
     }
 }
 __device__ __forceinline__ u32x4_t v_bf16(u32x4_t v) { return v; }
@@ -213,7 +287,7 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t x) {
 // the item the same of its rows together.
 template <int NT>
 struct Masks {
-  int L[NT], lo[NT], row[NT];  // columns of other rows: L = 0
+  int L[NT], lo[NT];  // columns of other rows: L = 0
   int sinks, Lmin, Lmax, lo_min, lo_max;
   bool rows;  // more than one
 };
@@ -298,7 +372,11 @@ __device__ __forceinline__ void take_odd(Tile<KV8>& b, const f32x4_t (&sacc)[NT]
 }
 
 // part_o [rows][Hq][NS][256] (unnormalised O), part_ml [rows][Hq][NS][2] = (max in log2 units, sum).
-template <int NT, bool KV8>
+// BATCH: persistent workgroups that take a part of the call's items each. While a wave computes the last tile of
+// an item, K of its first tile of the next one is on its way, and V during the merge of the four waves, so
+// that the memory latency of an item's begin is paid once per workgroup. Otherwise (few items) a workgroup is
+// an item: (slice, KV head; sequence), without the search for it.
+template <int NT, bool KV8, bool P16, bool BATCH>
 __global__ void __launch_bounds__(WAVES * WAVE) __attribute__((amdgpu_waves_per_eu(NT == 1 && KV8 ? 2 : 1, 2)))
 attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict__ kp,
                            const char* __restrict__ vp, const int* __restrict__ table,
@@ -306,17 +384,24 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
                            float* __restrict__ part_ml, Call a) {
   constexpr int LROW = KV8 ? 8 : 9;              // log2 of a cache row's bytes
   constexpr int SLOT = TILE << LROW;             // LDS bytes of a K tile
-  constexpr int WAREA = 2 * SLOT;                // a wave's two K slots
-  constexpr int MERGE = 16 * WAVE * 16;          // a wave's accumulators of one column tile
-  static_assert(WAREA >= MERGE, "the merge reuses the K slots");
-  __shared__ __attribute__((aligned(256))) char lds[WAVES * WAREA];
-  __shared__ float s_m[WAVES][16 * NT], s_l[WAVES][16 * NT];
+  // The merge takes rounds of MACC accumulators of one column tile per wave, through the K slot that the wave's
+  // last tile left. An fp8 slot holds half of them; with two column tiles, where registers allow one workgroup
+  // per CU, there is room for buffers of their own (16 sequences of 4 rows, 16 / 2 heads: 38 -> TODO us).
+  constexpr bool OWN = KV8 && NT == 2;
+  constexpr int HALVES = KV8 && !OWN ? 2 : 1, MACC = 16 / HALVES;
+  static_assert(OWN || MACC * WAVE * 16 == SLOT, "a round of the merge fills a K slot");
+  __shared__ __attribute__((aligned(256))) char lds[WAVES * (2 * SLOT + (OWN ? MACC * WAVE * 16 : 0))];
+  __shared__ __attribute__((aligned(16))) float s_ml[16 * NT][2][WAVES];  // (m, l) of a column's waves
+  __shared__ __attribute__((aligned(16))) uint32_t s_slot[WAVES];
   const int lane = threadIdx.x & (WAVE - 1);
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int w = uni(threadIdx.x / WAVE);
   const int c = lane & 15, g4 = lane >> 4;
   const int tc = blockIdx.y / a.hch * a.rc, hc = (blockIdx.y % a.hch) * a.hc;
   const int rn = min(a.rc, a.R - tc), hn = min(a.hc, a.grp - hc), ncols = rn * hn;
-  const uint32_t ks_s = lds_byte_uniform(lds + w * WAREA);
+  int i = (int)__umulhi(blockIdx.x, a.hkv_m);
+  if ((int)blockIdx.x - i * a.Hkv >= a.Hkv) ++i;
+  const int g = blockIdx.x - i * a.Hkv;
+  uint32_t cur = lds_byte_uniform(lds + w * 2 * SLOT), nxt = cur + SLOT;
   uint32_t kl, vl;
   if constexpr (KV8) {
     const TileLanes8 tl(lane);
@@ -325,28 +410,88 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
     const TileLanes tl(lane);
     kl = tl.kl, vl = tl.vl;
   }
+  Cursor cu;
+  if constexpr (BATCH) {
+    if (!first_item(a, pos, tc, rn, i, a.parts, lane, cu)) return;
+  } else {
+    const int p = pos_of(pos, blockIdx.z);
+    if (p < 0) return;
+    const int far = min(p + tc + rn, a.cap), ch = slice_size(a, far);
+    if (!a.window && ch == slice_size(a, min(p + tc + 1, a.cap))) {  // slice i, if it is there (cu.n: no further one)
+      if (i * ch >= far) return;
+      cu.k = cu.n = 0;
+      cu.it = Item{(int)blockIdx.z, p + tc, 0, rn, i, i * ch, min(i * ch + ch, far)};
+    } else {
+      open_sequence(a, cu, blockIdx.z, p, tc, rn);
+      if (i >= cu.n) return;
+      cu.k = i;
+      place_item(a, rn, cu);
+    }
+  }
+  Item it = cu.it;
 
-  bool again = false;
-  for (int x = blockIdx.x;; x += gridDim.x) {
-    int item = (int)__umulhi((uint32_t)x, a.hkv_m);
-    if (x - item * a.Hkv >= a.Hkv) ++item;
-    const int g = x - item * a.Hkv;
-    Item it;
-    if (!find_item(a, pos, tc, rn, item, lane, it)) return;
+  // Column ct*16+c is (row t, head g*grp + hc + j), col = t*hn + j; t = -1: padding
+  int trow[NT];
+#pragma unroll
+  for (int ct = 0; ct < NT; ++ct) {
+    const int col = ct * 16 + c;
+    trow[ct] = col < ncols ? col / hn : -1;
+  }
+  const int sinks = a.window ? a.sinks : 0;
 
-    // Q^T as the MFMA B operand: column ct*16+c is (row t, head g*grp + hc + j), col = t*hn + j
-    bf16x8_t qb[NT][8];
-    Masks<NT> mk;
+  // A wave's tiles of an item: j = beg / 32 + w, + 4, ..., without those wholly between the first tokens and
+  // the windows: the current one and the one after it, with the pages of their halves. Pages are read by scalar
+  // loads a tile ahead, where no LDS read is in flight (the two share a counter and return in no order).
+  struct Tiles {
+    int j, jn, jend, jlo;
+    int pg[2], pgn[2];
+  };
+  const auto skip = [&](int j, int jlo) __attribute__((always_inline)) {
+    return j < jlo && j * TILE >= sinks ? j + (jlo - j + WAVES - 1) / WAVES * WAVES : j;
+  };
+  const auto pages_of = [&](int (&pg)[2], int b, int j) __attribute__((always_inline)) {
+    const int* row = table + (size_t)b * a.ldt;
+    const int at = j * TILE >> a.lp;
+    pg[0] = row[min(at, a.M - 1)];
+    if constexpr (P16) pg[1] = at + 1 < a.M ? row[min(at + 1, a.M - 1)] : -1;
+  };
+  const auto tiles_of = [&](const Item& it) __attribute__((always_inline)) {
+    Tiles t;
+    t.jlo = a.window ? max(it.p0 + it.r0 + 1 - a.window, 0) / TILE : 0;
+    t.jend = (it.end + TILE - 1) / TILE;
+    t.j = skip(it.beg / TILE + w, t.jlo);
+    t.jn = skip(t.j + WAVES, t.jlo);
+    pages_of(t.pg, it.b, t.j);
+    pages_of(t.pgn, it.b, t.jn);
+    return t;
+  };
+  // resources of a tile in both pools; rows at or past the slice's end, or without a page, read 0. Returns the
+  // halves without a page.
+  const auto resources = [&](int j, int pgA, int pgB, int end, Rsrc& kr, Rsrc& vr)
+      __attribute__((always_inline)) {
+    constexpr int H = P16 ? 2 : 1, ROWS = TILE / H;
+    int bad = 0;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int pg = h ? pgB : pgA, ph = j * TILE + 16 * h;
+      const bool ok = (unsigned)pg < (unsigned)a.N;
+      bad |= ok ? 0 : P16 ? 1 << h : 3;
+      const int left = ok ? min(max(end - ph, 0), ROWS) : 0;
+      const size_t off = (((size_t)(ok ? pg : 0) * a.Hkv + g) << (a.lp + LROW)) +
+                         ((size_t)(ph & ((1 << a.lp) - 1)) << LROW);
+      kr.h[h] = make_rsrc_uniform(kp + off, (uint32_t)left << LROW);
+      vr.h[h] = make_rsrc_uniform(vp + off, (uint32_t)left << LROW);
+    }
+    return bad;
+  };
+  bf16x8_t qb[NT][8];  // Q^T as the MFMA B operand
+  const auto load_q = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) {
-      const int col = ct * 16 + c, t = col / hn, j = col - t * hn;
-      const bool mine = col < ncols && t >= it.r0 && t < it.r1;
-      mk.row[ct] = mine ? t : -1;
-      mk.L[ct] = mine ? min(it.p0 + t + 1, a.cap) : 0;
-      mk.lo[ct] = a.window ? it.p0 + t + 1 - a.window : 0;
-      if (col < ncols) {
+      const int t = trow[ct], j = ct * 16 + c - t * hn;
+      if (t >= 0) {
         const u32x4_t* src = reinterpret_cast<const u32x4_t*>(
-            q + ((size_t)(it.b * a.R + tc + t) * a.Hq + g * a.grp + hc + j) * HD);
+            q + ((size_t)(b * a.R + tc + t) * a.Hq + g * a.grp + hc + j) * HD);
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) qb[ct][ks] = as_bf16x8(src[4 * ks + g4]);
       } else {
@@ -354,45 +499,57 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
         for (int ks = 0; ks < 8; ++ks) qb[ct][ks] = as_bf16x8(u32x4_t{0u, 0u, 0u, 0u});
       }
     }
+  };
+
+  Tile<KV8> buf;
+  Rsrc kr, vr;
+  int bad = 0;
+  Tiles ti;
+  bool on;  // the wave has a tile of the item, and it is on its way
+  const auto begin = [&]() __attribute__((always_inline)) {
+    ti = tiles_of(it);
+    on = ti.j < ti.jend;
+    if (BATCH || on) {
+      bad = resources(ti.j, ti.pg[0], ti.pg[1], on ? it.end : 0, kr, vr);
+      issue_k<KV8, P16>(cur, kr, kl);
+      __builtin_amdgcn_sched_barrier(0);
+      issue_v<KV8, P16>(buf, vr, vl);
+    }
+  };
+  bool merged = false;  // since the last barrier
+  load_q(it.b);  // ahead of the tiles' loads: a wait for it is none for them
+  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (BATCH) begin();
+
+  for (;;) {
+    // the next item, and this wave's first tiles in it
+    bool more_items = false;
+    Item it2 = it;
+    Tiles t2{};
+    if constexpr (BATCH) {
+      ++cu.k;
+      more_items = take_item(a, pos, tc, rn, cu);
+      it2 = cu.it;
+      if (more_items) t2 = tiles_of(it2);
+    } else {
+      if (merged) lds_barrier();  // every wave has read the merge's slots
+      begin();
+    }
+    const bool on2 = t2.j < t2.jend;
+
+    Masks<NT> mk;
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
+      const int t = trow[ct];
+      const bool mine = t >= it.r0 && t < it.r1;
+      mk.L[ct] = mine ? min(it.p0 + t + 1, a.cap) : 0;
+      mk.lo[ct] = a.window ? it.p0 + t + 1 - a.window : 0;
+    }
     mk.rows = it.r1 - it.r0 > 1;
     mk.Lmin = min(it.p0 + it.r0 + 1, a.cap), mk.Lmax = min(it.p0 + it.r1, a.cap);
     mk.lo_min = a.window ? it.p0 + it.r0 + 1 - a.window : 0;
     mk.lo_max = a.window ? it.p0 + it.r1 - a.window : 0;
-    mk.sinks = a.window ? a.sinks : 0;
-
-    // The wave's tiles: j = beg / 32 + w, + 4, ..., without those wholly between the first tokens and the
-    // windows. Lane i holds the pages of the halves of tile jb + 4 i.
-    const int* trow = table + (size_t)it.b * a.ldt;
-    const int jlo = max(mk.lo_min, 0) / TILE, jend = (it.end + TILE - 1) / TILE;
-    const auto skip = [&](int j) __attribute__((always_inline)) {
-      return j < jlo && j * TILE >= mk.sinks ? j + (jlo - j + WAVES - 1) / WAVES * WAVES : j;
-    };
-    int j = skip(it.beg / TILE + w);
-    int jb = 0, pgA = 0, pgB = 0;
-    const auto pages_from = [&](int j0) __attribute__((always_inline)) {
-      jb = j0;
-      const int p = (j0 + WAVES * lane) * TILE;
-      const int ia = p >> a.lp, ib = (p + 16) >> a.lp;
-      pgA = ia < a.M ? trow[ia] : -1;
-      pgB = ib < a.M ? trow[ib] : -1;
-    };
-    // resources of tile j's halves in both pools; rows at or past the slice's end read 0
-    const auto halves = [&](int j, Halves& kh, Halves& vh) __attribute__((always_inline)) {
-      const int at = (j - jb) / WAVES, p = j * TILE;
-      int bad = 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int pg = __builtin_amdgcn_readlane(h ? pgB : pgA, at);
-        const bool ok = (unsigned)pg < (unsigned)a.N;
-        bad |= ok ? 0 : 1 << h;
-        const int ph = p + 16 * h, left = ok ? min(max(it.end - ph, 0), 16) : 0;
-        const size_t off = (((size_t)(ok ? pg : 0) * a.Hkv + g) << (a.lp + LROW)) +
-                           ((size_t)(ph & ((1 << a.lp) - 1)) << LROW);
-        kh.h[h] = make_rsrc_uniform(kp + off, (uint32_t)left << LROW);
-        vh.h[h] = make_rsrc_uniform(vp + off, (uint32_t)left << LROW);
-      }
-      return bad;
-    };
+    mk.sinks = sinks;
 
     float m[NT], l[NT];
     f32x4_t acc[NT][16];  // [8hh + i]: O^T dims 128hh + 32g4 + 8ii + i (tile::pv_half)
@@ -403,13 +560,9 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[ct][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-    if (again) lds_barrier();  // the previous item's merge has read every wave's slots
-    again = true;
-
-    Tile<KV8> buf;
-    const auto compute = [&](uint32_t slot, int j, int bad) __attribute__((always_inline)) {
+    const auto compute = [&](bool last) __attribute__((always_inline)) {
       const u32x4_t* kt =
-          (const u32x4_t*)((__attribute__((address_space(3))) const u32x4_t*)(uintptr_t)slot);
+          (const u32x4_t*)((__attribute__((address_space(3))) const u32x4_t*)(uintptr_t)cur);
       wave_lds_fence();
       f32x4_t sacc[NT][2];
       if constexpr (KV8)
@@ -417,7 +570,12 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
       else
         tile::qk_tile<NT, NT == 1, NT == 2 ? 2 : 0>(kt, qb, c, g4, sacc);
       wave_lds_fence();
-      const int p = j * TILE;
+      const int p = ti.j * TILE;
+      if (!last) {
+        ti.j = ti.jn;
+        ti.jn = skip(ti.jn + WAVES, ti.jlo);
+        pages_of(ti.pgn, it.b, ti.jn);
+      }
       if (p + TILE > mk.Lmin || bad || (p < mk.lo_max && p + TILE > mk.sinks)) {
         if (mask_tile<NT, KV8>(buf, sacc, p, bad, mk, g4)) take_odd<NT, KV8>(buf, sacc, acc);
       }
@@ -426,145 +584,243 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
       tile::softmax_tile<NT, false, true>(sacc, p, none, a.scale_log2, g4, m, l, acc, pb_hi, pb_lo);
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
-        u32x4_t vr[8];
+        u32x4_t rows[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) vr[e] = v_bf16(buf.v[e][hh]);
-        tile::pv_half<NT, true>(vr, hh, pb_hi, pb_lo, acc);
+        for (int e = 0; e < 8; ++e) rows[e] = v_bf16(buf.v[e][hh]);
+        tile::pv_half<NT, true>(rows, hh, pb_hi, pb_lo, acc);
       }
     };
-    if (j < jend) {
-      pages_from(j);
-      uint32_t cur = ks_s, nxt = ks_s + SLOT;
-      Halves kh, vh;
-      int bad = halves(j, kh, vh);
-      issue_k<KV8>(cur, kh, kl);
-      __builtin_amdgcn_sched_barrier(0);
-      issue_v<KV8>(buf, vh, vl);
+    // K of a tile has landed when at most 16 loads are under way: its V was issued after it. The compiler's
+    // waits for V count on the K loads behind it, so a loop issues both in every step (of a wave that has no
+    // further tile, with empty resources) or is left before its last tile.
+    if constexpr (BATCH) {
       for (;;) {
-        const int jn = skip(j + WAVES);
-        const bool more = jn < jend;  // uniform
-        int bad_n = 0;
-        if (more) {
-          if (jn - jb >= WAVES * WAVE) pages_from(jn);
-          bad_n = halves(jn, kh, vh);
+        // the tile after this one: of this item, or the first of the next
+        const bool last = !on || ti.jn >= ti.jend;
+        const int bad_n = resources(last ? t2.j : ti.jn, last ? t2.pg[0] : ti.pgn[0],
+                                    last ? t2.pg[1] : ti.pgn[1], last ? (on2 ? it2.end : 0) : it.end, kr, vr);
+        vmcnt_wait<16>();
+        if (merged) lds_barrier();  // every wave has read the merge's slots, which the tiles go to again
+        merged = false;
+        __builtin_amdgcn_sched_barrier(0);
+        issue_k<KV8, P16>(nxt, kr, kl);
+        __builtin_amdgcn_sched_barrier(0);
+        if (on) compute(last);
+        __builtin_amdgcn_sched_barrier(0);
+        if (last && more_items && it2.b != it.b) {
+          load_q(it2.b);
+          // waited for here, not by every tile of the loop
+#pragma unroll
+          for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) asm volatile("" : "+v"(qb[ct][ks]));
         }
-        vmcnt_wait<16>();  // this tile's K: its V (16 loads) may remain
         __builtin_amdgcn_sched_barrier(0);
-        if (more) issue_k<KV8>(nxt, kh, kl);
-        __builtin_amdgcn_sched_barrier(0);
-        compute(cur, j, bad);
-        __builtin_amdgcn_sched_barrier(0);
-        if (!more) break;
-        issue_v<KV8>(buf, vh, vl);
-        j = jn, bad = bad_n;
+        issue_v<KV8, P16>(buf, vr, vl);
+        bad = bad_n;
+        if (last) break;
         const uint32_t t = cur;
         cur = nxt, nxt = t;
       }
+    } else if (on) {
+      while (ti.jn < ti.jend) {
+        const int bad_n = resources(ti.jn, ti.pgn[0], ti.pgn[1], it.end, kr, vr);
+        vmcnt_wait<16>();
+        __builtin_amdgcn_sched_barrier(0);
+        issue_k<KV8, P16>(nxt, kr, kl);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(false);
+        __builtin_amdgcn_sched_barrier(0);
+        issue_v<KV8, P16>(buf, vr, vl);
+        bad = bad_n;
+        const uint32_t t = cur;
+        cur = nxt, nxt = t;
+      }
+      vmcnt_wait<16>();
+      compute(true);
     }
 
-    // ---- merge the waves in order 0..3 and write the slice's partial
-#pragma unroll
-    for (int ct = 0; ct < NT; ++ct) {
-      l[ct] = group4_sum(l[ct]);
-      if (g4 == 0) {
-        s_m[w][ct * 16 + c] = m[ct];
-        s_l[w][ct * 16 + c] = l[ct];
-      }
-    }
-    const auto s_acc = [&](int v, int i) __attribute__((always_inline)) -> f32x4_t& {
-      return reinterpret_cast<f32x4_t*>(lds + v * WAREA)[i * WAVE + lane];
+    // ---- the slice's partial
+    // a row's slot; without a window slice i's is i
+    const auto slot = [&](int ct) __attribute__((always_inline)) {
+      const int t = trow[ct];
+      int sl = -1;
+      if (t >= it.r0 && t < it.r1)
+        sl = !a.window ? (it.beg < mk.L[ct] ? it.slice : -1) : slot_of(row_slices(a, it.p0 + t), it.slice);
+      return sl < a.NS ? sl : -1;
+    };
+    const auto place = [&](int ct, int sl) __attribute__((always_inline)) {
+      const int t = trow[ct], head = g * a.grp + hc + (ct * 16 + c - t * hn);
+      return ((size_t)(it.b * a.R + tc + t) * a.Hq + head) * a.NS + sl;
     };
 #pragma unroll
-    for (int ct = 0; ct < NT; ++ct) {
-      const int t = mk.row[ct];
-      if (ct > 0) lds_barrier();  // the previous column tile's reads are done
-      if (t >= 0) {
+    for (int ct = 0; ct < NT; ++ct) l[ct] = group4_sum(l[ct]);
+    merged = it.end - it.beg > TILE;
+    if (!merged) {
+      // one tile: the other waves hold m = -inf, l = 0, O = 0, so that wave 0's are the partial, bit for bit
+      if (w == 0) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s_acc(w, i) = acc[ct][i];
+        for (int ct = 0; ct < NT; ++ct) {
+          const int sl = slot(ct);
+          if (sl < 0) continue;
+          const size_t at = place(ct, sl);
+          if (g4 == 0) *reinterpret_cast<float2*>(part_ml + 2 * at) = make_float2(m[ct], l[ct]);
+          float* dst = part_o + at * HD + 32 * g4;
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int ii = 0; ii < 4; ++ii)
+#pragma unroll
+              for (int i = 0; i < 8; i += 4)
+                *reinterpret_cast<f32x4_t*>(dst + 128 * hh + 8 * ii + i) =
+                    f32x4_t{acc[ct][8 * hh + i][ii], acc[ct][8 * hh + i + 1][ii], acc[ct][8 * hh + i + 2][ii],
+                            acc[ct][8 * hh + i + 3][ii]};
+        }
       }
-      lds_barrier();
-      const int sl = t < 0 ? -1 : slot_of(row_slices(a, it.p0 + t), it.slice);
-      if (sl >= 0 && sl < a.NS) {
-        const int col = ct * 16 + c;
-        float M = -INFINITY, wsc[WAVES], L = 0.f;
+    } else {
+      // the waves' merge, in order 0..3
+      const uint32_t park = OWN ? lds_byte_uniform(lds + WAVES * 2 * SLOT + w * (MACC * WAVE * 16)) : cur;
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) M = fmaxf(M, s_m[v][col]);
+      for (int ct = 0; ct < NT; ++ct)
+        if (g4 == 0) s_ml[ct * 16 + c][0][w] = m[ct], s_ml[ct * 16 + c][1][w] = l[ct];
+      if (lane == 0) s_slot[w] = park;
+      const auto s_acc = [&](uint32_t at, int i) __attribute__((always_inline)) {
+        return (__attribute__((address_space(3))) f32x4_t*)(uintptr_t)(at + i * (WAVE * 16));
+      };
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) {
-          const float mv = s_m[v][col];
-          wsc[v] = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - M);
-          L += s_l[v][col] * wsc[v];
+      for (int ct = 0; ct < NT; ++ct) {
+        const int sl = slot(ct);
+#pragma unroll
+        for (int hf = 0; hf < HALVES; ++hf) {
+          if (ct > 0 || hf > 0) lds_barrier();  // the previous round's reads are done
+          if (trow[ct] >= it.r0 && trow[ct] < it.r1) {
+#pragma unroll
+            for (int i = 0; i < MACC; ++i) *s_acc(park + lane * 16, i) = acc[ct][MACC * hf + i];
+          }
+          lds_barrier();
+          if (sl >= 0) {
+            const f32x4_t mv = *reinterpret_cast<const f32x4_t*>(s_ml[ct * 16 + c][0]);
+            const f32x4_t lv = *reinterpret_cast<const f32x4_t*>(s_ml[ct * 16 + c][1]);
+            const u32x4_t from = *reinterpret_cast<const u32x4_t*>(s_slot) + (uint32_t)(lane * 16);
+            const float M = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3]));
+            float wsc[WAVES], L = 0.f;
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) {
+              wsc[v] = mv[v] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv[v] - M);
+              L = __builtin_fmaf(lv[v], wsc[v], L);
+            }
+            const size_t at = place(ct, sl);
+            if (w == 0 && g4 == 0 && hf == 0)
+              *reinterpret_cast<float2*>(part_ml + 2 * at) = make_float2(M, L);
+            // this thread's accumulators: the i-th of each half (128 dims), i0 .. i0 + PER
+            constexpr int PER = MACC / WAVES;
+            const int h = HALVES == 2 ? hf : w >> 1, i0 = HALVES == 2 ? PER * w : PER * (w & 1);
+            const int k0 = HALVES == 2 ? i0 : 8 * h + i0;
+            f32x4_t mo[PER];
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+              f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int v = 0; v < WAVES; ++v) {
+                const f32x4_t x = *s_acc(from[v] + k0 * (WAVE * 16), k);
+#pragma unroll
+                for (int ii = 0; ii < 4; ++ii) sum[ii] = __builtin_fmaf(x[ii], wsc[v], sum[ii]);
+              }
+              mo[k] = sum;
+            }
+            float* dst = part_o + at * HD + 128 * h + 32 * g4 + i0;
+#pragma unroll
+            for (int ii = 0; ii < 4; ++ii) {
+              if constexpr (PER == 4)
+                *reinterpret_cast<f32x4_t*>(dst + 8 * ii) = f32x4_t{mo[0][ii], mo[1][ii], mo[2][ii], mo[3][ii]};
+              else
+                *reinterpret_cast<float2*>(dst + 8 * ii) = make_float2(mo[0][ii], mo[1][ii]);
+            }
+          }
         }
-        const int head = g * a.grp + hc + (col - t * hn);
-        const size_t at = ((size_t)(it.b * a.R + tc + t) * a.Hq + head) * a.NS + sl;
-        if (w == 0 && g4 == 0) {
-          part_ml[2 * at] = M;
-          part_ml[2 * at + 1] = L;
-        }
-        const int h = w >> 1, i0 = 4 * (w & 1);
-        f32x4_t mo[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int v = 0; v < WAVES; ++v) sum += s_acc(v, 8 * h + i0 + k) * wsc[v];
-          mo[k] = sum;
-        }
-        float* dst = part_o + at * HD + 128 * h + 32 * g4 + i0;
-#pragma unroll
-        for (int ii = 0; ii < 4; ++ii)
-          reinterpret_cast<f32x4_t*>(dst + 8 * ii)[0] =
-              f32x4_t{mo[0][ii], mo[1][ii], mo[2][ii], mo[3][ii]};
       }
+    }
+    if constexpr (BATCH) {
+      if (!more_items) {
+        vmcnt_wait<0>();  // no LDS DMA may still target this workgroup's LDS
+        return;
+      }
+      if (on2) {
+        const uint32_t t = cur;
+        cur = nxt, nxt = t;
+      }
+      it = it2, ti = t2, on = on2;
+    } else {
+      cu.k += a.parts;  // (more items than slots: rows with two slice sizes)
+      if (cu.k >= cu.n) return;
+      place_item(a, rn, cu);
+      it = cu.it;
     }
   }
 }
 
-// Merge of a row's slices and the gate: one wave per (head, row, 16 dims), lane = (slot group g of 16,
-// 4 dims). A group takes slots s0 + 16 i + g; the groups meet in a fixed tree.
-constexpr int CDIMS = 16;
-__device__ __forceinline__ float group16_sum(float v) {
-  v = xor16_pair(xor32_pair(v, true), true);
-  v = v + dpp<0x128>(v);
-  return v + dpp<0x1B>(dpp<0x141>(v));
+// Merge of a row's slices and the gate. A wave takes 256 / G dims of a (head, row): G groups of lanes, lane =
+// (group, 4 dims); a group takes slots s0 + G i + group, and the groups meet in a fixed tree. AHEAD: the first
+// G * U slots are loaded before the position arrives (clamped to the row's slots, those that do not count
+// are selected away): one memory round trip less where the loads are few.
+template <int G>
+__device__ __forceinline__ float groups(float v, bool sum) {
+  const auto op = [&](float x, float y) __attribute__((always_inline)) { return sum ? x + y : fmaxf(x, y); };
+  v = xor32_pair(v, sum);
+  v = xor16_pair(v, sum);
+  if constexpr (G == 16) {
+    v = op(v, dpp<0x128>(v));               // lane ^ 8
+    v = op(v, dpp<0x1B>(dpp<0x141>(v)));    // lane ^ 4
+  }
+  return v;
 }
-__device__ __forceinline__ float group16_max(float v) {
-  v = fmaxf(v, dpp<0x128>(v));
-  v = fmaxf(v, dpp<0x1B>(dpp<0x141>(v)));
-  return xor32_pair(xor16_pair(v, false), false);
-}
+template <int G, bool AHEAD>
 __global__ void __launch_bounds__(WAVES * WAVE)
 attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
                           const int* __restrict__ pos, const __bf16* __restrict__ qg,
                           __bf16* __restrict__ out, Call a) {
-  constexpr int G = 16, U = 4;
-  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE, cd = lane & 3, g = lane >> 2;
-  const int h = blockIdx.x, row = blockIdx.y, dim = (blockIdx.z * WAVES + w) * CDIMS + 4 * cd;
+  constexpr int U = 4, LD = WAVE / G;  // slots in flight per group, lanes of a group
+  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE, g = lane / LD;
+  // waves: (row, head, chunk of dims), the chunk fastest
+  const int id = blockIdx.x * WAVES + w, dim = (id % G) * (4 * LD) + 4 * (lane % LD);
+  const int rh = id / G, row = (int)((unsigned)rh / (unsigned)a.Hq), h = rh - row * a.Hq;
+  if (row >= a.B * a.R) return;
   const int b = row / a.R, t = row - b * a.R;
-  const int p0 = pos_of(pos, b);
-  if (p0 < 0) return;
+  const size_t base = ((size_t)row * a.Hq + h) * a.NS;
+  f32x4_t po[U];
+  float2 ml[U];
+  const auto load = [&](int s0, int n) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (i > 0 && s0 + G * i >= n) break;  // uniform
+      const int s = min(s0 + G * i + g, n - 1);
+      po[i] = *reinterpret_cast<const f32x4_t*>(part_o + (base + s) * HD + dim);
+      ml[i] = *reinterpret_cast<const float2*>(part_ml + 2 * (base + s));
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    po[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    ml[i] = make_float2(-INFINITY, 0.f);
+  }
   const __bf16* gp = qg + (size_t)row * a.ldp + (size_t)h * 2 * HD + HD + dim;
   float gate[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) gate[i] = bf16_to_f32(gp[i]);
+  if constexpr (AHEAD) load(0, a.NS);
+  const int p0 = pos_of(pos, b);
+  if (p0 < 0) return;
   const int cnt = min(row_slices(a, p0 + t).cnt, a.NS);
-  const size_t base = ((size_t)row * a.Hq + h) * a.NS;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) gate[i] = sigmoid_f32(gate[i]);
   f32x4_t O = {0.f, 0.f, 0.f, 0.f};
   float L = 0.f, M = -INFINITY;
   for (int s0 = 0; s0 < cnt; s0 += G * U) {
-    f32x4_t po[U];
-    float2 ml[U];
+    if (!AHEAD || s0 > 0) load(s0, cnt);
+    float mv[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int s = s0 + G * i + g;
-      po[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      ml[i] = make_float2(-INFINITY, 0.f);
-      if (s < cnt) {
-        po[i] = *reinterpret_cast<const f32x4_t*>(part_o + (base + s) * HD + dim);
-        ml[i] = *reinterpret_cast<const float2*>(part_ml + 2 * (base + s));
-      }
-    }
-    const float bm = group16_max(fmaxf(M, fmaxf(fmaxf(ml[0].x, ml[2].x), fmaxf(ml[1].x, ml[3].x))));
+    for (int i = 0; i < U; ++i) mv[i] = s0 + G * i + g < cnt ? ml[i].x : -INFINITY;
+    const float bm = groups<G>(fmaxf(M, fmaxf(fmaxf(mv[0], mv[2]), fmaxf(mv[1], mv[3]))), false);
     if (bm != M) {
       const float r = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - bm);
       O *= r;
@@ -573,21 +829,21 @@ attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restr
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const bool use = ml[i].x != -INFINITY;
-      const float f = use ? __builtin_amdgcn_exp2f(ml[i].x - M) : 0.f;
+      const bool use = mv[i] != -INFINITY;
+      const float f = use ? __builtin_amdgcn_exp2f(mv[i] - M) : 0.f;
       const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
       L += (use ? ml[i].y : 0.f) * f;
       O += (use ? po[i] : zero) * f;
     }
   }
-  L = group16_sum(L);
+  L = groups<G>(L, true);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) O[i] = group16_sum(O[i]);
+  for (int i = 0; i < 4; ++i) O[i] = groups<G>(O[i], true);
   if (g == 0) {
     __bf16* op = out + (size_t)row * a.ldo + (size_t)h * HD + dim;
 #pragma unroll
     for (int i = 0; i < 4; ++i)  // a row that attends nothing: 0
-      op[i] = f32_to_bf16(L == 0.f ? 0.f : (O[i] / L) * a.v_scale * sigmoid_f32(gate[i]));
+      op[i] = f32_to_bf16(L == 0.f ? 0.f : (O[i] / L) * a.v_scale * gate[i]);
   }
 }
 
@@ -626,19 +882,40 @@ static hipError_t launch(const void* q, const void* kp, const void* vp, const in
   a.hkv_m = Hkv == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (unsigned)Hkv);
   a.ldt = ldt, a.ldp = ldp, a.ldo = ldo;
   a.scale_log2 = scale * 1.4426950408889634f, a.v_scale = v_scale;
+  // as many workgroups as run at once: 128 KB of LDS each, or 64 KB and 256 registers
+  const int NT = a.rc * a.hc <= 16 ? 1 : 2, at_once = compute_units() * (KV8 && NT == 1 ? 2 : 1);
   const long slices = window ? NS : std::min<long>(NS, (a.cap + a.mins - 1) / a.mins);
-  const unsigned items = (unsigned)std::min<long>((long)B * slices * Hkv, 4l * compute_units());
-  const dim3 grid(items, rch * a.hch), block(WAVES * WAVE);
+  const bool batch = B * slices * Hkv > 2 * compute_units();
+  a.parts = batch ? std::max(1, at_once / Hkv) : (int)slices;
+  const dim3 grid((unsigned)(a.parts * Hkv), rch * a.hch, batch ? 1 : B), block(WAVES * WAVE);
   const auto* Q = static_cast<const __bf16*>(q);
   const auto *K = static_cast<const char*>(kp), *V = static_cast<const char*>(vp);
-  if (a.rc * a.hc <= 16)
-    attn_paged_partials_kernel<1, KV8><<<grid, block, 0, stream>>>(Q, K, V, table, pos, part_o, part_ml, a);
-  else
-    attn_paged_partials_kernel<2, KV8><<<grid, block, 0, stream>>>(Q, K, V, table, pos, part_o, part_ml, a);
+  const auto go = [&](auto nt, auto p16, auto bt) {
+    attn_paged_partials_kernel<decltype(nt)::value, KV8, decltype(p16)::value, decltype(bt)::value>
+        <<<grid, block, 0, stream>>>(Q, K, V, table, pos, part_o, part_ml, a);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  const auto by_page = [&](auto nt, auto bt) {
+    P == 16 ? go(nt, std::true_type{}, bt) : go(nt, std::false_type{}, bt);
+  };
+  const auto by_batch = [&](auto nt) {
+    batch ? by_page(nt, std::true_type{}) : by_page(nt, std::false_type{});
+  };
+  NT == 1 ? by_batch(One{}) : by_batch(Two{});
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  attn_paged_combine_kernel<<<dim3(Hq, B * R, HD / CDIMS / WAVES), block, 0, stream>>>(
-      part_o, part_ml, pos, static_cast<const __bf16*>(qg), static_cast<__bf16*>(out), a);
+  const long heads = (long)B * R * Hq;
+  const auto merge = [&](auto G, auto ahead) {
+    constexpr int g = decltype(G)::value;
+    attn_paged_combine_kernel<g, decltype(ahead)::value>
+        <<<dim3((unsigned)((heads * g + WAVES - 1) / WAVES)), block, 0, stream>>>(
+            part_o, part_ml, pos, static_cast<const __bf16*>(qg), static_cast<__bf16*>(out), a);
+  };
+  if (batch)
+    merge(std::integral_constant<int, 4>{}, std::false_type{});
+  else
+    merge(std::integral_constant<int, 16>{}, std::true_type{});
   return hipGetLastError();
 }
 
