@@ -149,13 +149,6 @@ struct Cursor {
   int ch, nsk, wlo, lo;  // the first row's slices
   int at, len, hi;       // (parts of a line, below)
 };
-__device__ __forceinline__ SeqItems open_sequence(const Call& a, Cursor& c, int b, int p, int tc, int rn) {
-  c.it.b = b, c.it.p0 = p + tc;
-  const SeqItems q = seq_items(a, c.it.p0, rn);
-  c.k = 0, c.nA = uni(q.nA), c.n = uni(q.n), c.tB = uni(q.tB);
-  c.ch = uni(q.f.ch), c.nsk = uni(q.f.nsk), c.wlo = uni(q.f.wlo), c.lo = uni(q.f.lo);
-  return q;
-}
 __device__ __forceinline__ void place_item(const Call& a, int rn, Cursor& c) {
   int k = c.k, nsk = c.nsk, wlo = c.wlo, ch = c.ch;
   c.it.r0 = 0, c.it.r1 = c.tB;
@@ -186,56 +179,89 @@ __device__ __forceinline__ int place_of(const Call& a, const Cursor& c) {
                         : a.sinks / TILE + 1 + max((c.wlo + c.k - c.nsk) * c.ch - c.lo, 0) / TILE;
   return c.at + min(c.k * OVER + tiles, c.len - 1);
 }
-__device__ __forceinline__ void open_on_line(const Call& a, Cursor& c, int b, int p, int tc, int rn) {
-  const SeqItems q = open_sequence(a, c, b, p, tc, rn);
-  c.len = uni(line_of(a, q, c.it.p0, rn));
+
+// The call's sequences as a wave holds them: up to 64, one a lane, with their items. Beyond that a lane has several
+// consecutive ones and only their length on the line; an item's sequence is then looked up again.
+struct Lanes {
+  int K;                 // sequences a lane
+  int p, n, nA, tB, ch, nsk, wlo, lo, len;  // (one a lane) of its sequence; p < 0: idle
+  int upto;              // place on the line where the lane's sequences end
+};
+__device__ __forceinline__ void lane_seq(const Call& a, Lanes& l, int p, int rn) {
+  const SeqItems q = seq_items(a, p, rn);
+  l.n = q.n, l.nA = q.nA, l.tB = q.tB;
+  l.ch = q.f.ch, l.nsk = q.f.nsk, l.wlo = q.f.wlo, l.lo = q.f.lo;
+  l.len = line_of(a, q, p, rn);
+}
+__device__ __forceinline__ Lanes lanes_of(const Call& a, const int* pos, int tc, int rn, int lane) {
+  Lanes l{};
+  l.K = (a.B + WAVE - 1) / WAVE;
+  l.p = -1;
+  int mine = 0;
+  for (int s = 0; s < l.K; ++s) {
+    const int b = lane * l.K + s;
+    l.p = b < a.B ? pos_of(pos, b) : -1;
+    l.n = l.len = 0;
+    if (l.p >= 0) lane_seq(a, l, l.p += tc, rn);
+    mine += l.len;
+  }
+  l.upto = wave_scan(mine);
+  return l;
+}
+// Opens sequence b at its item 0; false if it is idle.
+__device__ __forceinline__ bool open_sequence(const Call& a, const Lanes& l, const int* pos, int tc, int rn, int b,
+                                              Cursor& c) {
+  const auto at = [&](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(x, b); };
+  c.it.b = b, c.k = 0;
+  if (l.K == 1) {
+    c.it.p0 = at(l.p), c.n = at(l.n), c.nA = at(l.nA), c.tB = at(l.tB);
+    c.ch = at(l.ch), c.nsk = at(l.nsk), c.wlo = at(l.wlo), c.lo = at(l.lo), c.len = at(l.len);
+    return c.it.p0 >= 0;
+  }
+  const int p = uni(pos_of(pos, b));
+  if (p < 0) {
+    c.n = c.len = 0;
+    return false;
+  }
+  Lanes one{};
+  lane_seq(a, one, p + tc, rn);
+  c.it.p0 = p + tc, c.n = uni(one.n), c.nA = uni(one.nA), c.tB = uni(one.tB);
+  c.ch = uni(one.ch), c.nsk = uni(one.nsk), c.wlo = uni(one.wlo), c.lo = uni(one.lo), c.len = uni(one.len);
+  return true;
 }
 // The cursor's item, if it begins in the part. At the end of a sequence: the next one's first.
-__device__ __forceinline__ bool take_item(const Call& a, const int* pos, int tc, int rn, Cursor& c) {
+__device__ __forceinline__ bool take_item(const Call& a, const Lanes& l, const int* pos, int tc, int rn,
+                                          Cursor& c) {
   while (c.k >= c.n) {
     c.at += c.len;
-    int b = c.it.b, p = -1;
-    while (p < 0) {
-      if (++b >= a.B) return false;
-      p = pos_of(pos, uni(b));
-    }
-    open_on_line(a, c, b, p, tc, rn);
+    const int b = c.it.b + 1;
+    if (b >= a.B) return false;
+    open_sequence(a, l, pos, tc, rn, b, c);  // (an idle one has no items)
   }
   if (place_of(a, c) >= c.hi) return false;
   place_item(a, rn, c);
   return true;
 }
 // The first item of part i of `parts`.
-__device__ __forceinline__ bool first_item(const Call& a, const int* pos, int tc, int rn, int i, int parts,
-                                           int lane, Cursor& c) {
-  const int K = (a.B + WAVE - 1) / WAVE;  // sequences per lane, consecutive
-  int mine = 0, p = -1;
-  for (int s = 0; s < K; ++s) {
-    const int b = lane * K + s;
-    p = b < a.B ? pos_of(pos, b) : -1;
-    if (p >= 0) mine += line_of(a, seq_items(a, p + tc, rn), p + tc, rn);
-  }
-  const int upto = wave_scan(mine);
-  const int total = __builtin_amdgcn_readlane(upto, WAVE - 1);
+__device__ __forceinline__ bool first_item(const Call& a, const Lanes& l, const int* pos, int tc, int rn, int i,
+                                           int parts, Cursor& c) {
+  const int total = __builtin_amdgcn_readlane(l.upto, WAVE - 1);
   const int part = uni((int)(((unsigned)total + parts - 1) / (unsigned)parts)), lo = i * part;
   c.hi = min(part, total - lo);
-  const int at = __popcll(__ballot(upto <= lo));  // the lane whose sequences hold the part's begin
+  const int at = __popcll(__ballot(l.upto <= lo));  // the lane whose sequences hold the part's begin
   if (lo >= total || at >= WAVE) return false;
-  c.at = __builtin_amdgcn_readlane(upto - mine, at) - lo;
+  c.at = (at > 0 ? __builtin_amdgcn_readlane(l.upto, at - 1) : 0) - lo;
   for (int s = 0;; ++s) {
-    const int b = at * K + s;
-    if (s >= K || b >= a.B) return false;  // (pos changed meanwhile)
-    const int q = K == 1 ? __builtin_amdgcn_readlane(p, at) : uni(pos_of(pos, b));
-    if (q < 0) continue;
-    open_on_line(a, c, b, q, tc, rn);
-    if (c.at + c.len > 0) break;
+    const int b = at * l.K + s;
+    if (s >= l.K || b >= a.B) return false;  // (pos changed meanwhile)
+    if (open_sequence(a, l, pos, tc, rn, b, c) && c.at + c.len > 0) break;
     c.at += c.len;
   }
   // the first item from the part's begin on: an estimate, then steps
   c.k = min(max(-c.at, 0) / (c.ch / TILE + OVER), c.n);
   while (c.k > 0 && (c.k >= c.n || place_of(a, c) >= 0)) --c.k;
   while (c.k < c.n && place_of(a, c) < 0) ++c.k;
-  return take_item(a, pos, tc, rn, c);
+  return take_item(a, l, pos, tc, rn, c);
 }
 
 // ---- a tile of the paged cache: one buffer resource, or with pages of 16 positions (P16) one for each half
@@ -386,7 +412,7 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
   constexpr int SLOT = TILE << LROW;             // LDS bytes of a K tile
   // The merge takes rounds of MACC accumulators of one column tile per wave, through the K slot that the wave's
   // last tile left. An fp8 slot holds half of them; with two column tiles, where registers allow one workgroup
-  // per CU, there is room for buffers of their own (16 sequences of 4 rows, 16 / 2 heads: 38 -> TODO us).
+  // per CU, there is room for buffers of their own (16 sequences of 4 rows, 16 / 2 heads: 38 -> 34 us).
   constexpr bool OWN = KV8 && NT == 2;
   constexpr int HALVES = KV8 && !OWN ? 2 : 1, MACC = 16 / HALVES;
   static_assert(OWN || MACC * WAVE * 16 == SLOT, "a round of the merge fills a K slot");
@@ -411,8 +437,10 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
     kl = tl.kl, vl = tl.vl;
   }
   Cursor cu;
+  Lanes lanes{};
   if constexpr (BATCH) {
-    if (!first_item(a, pos, tc, rn, i, a.parts, lane, cu)) return;
+    lanes = lanes_of(a, pos, tc, rn, lane);
+    if (!first_item(a, lanes, pos, tc, rn, i, a.parts, cu)) return;
   } else {
     const int p = pos_of(pos, blockIdx.z);
     if (p < 0) return;
@@ -422,7 +450,10 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
       cu.k = cu.n = 0;
       cu.it = Item{(int)blockIdx.z, p + tc, 0, rn, i, i * ch, min(i * ch + ch, far)};
     } else {
-      open_sequence(a, cu, blockIdx.z, p, tc, rn);
+      const SeqItems q = seq_items(a, p + tc, rn);
+      cu.it.b = blockIdx.z, cu.it.p0 = p + tc;
+      cu.nA = uni(q.nA), cu.n = uni(q.n), cu.tB = uni(q.tB);
+      cu.ch = uni(q.f.ch), cu.nsk = uni(q.f.nsk), cu.wlo = uni(q.f.wlo);
       if (i >= cu.n) return;
       cu.k = i;
       place_item(a, rn, cu);
@@ -528,7 +559,7 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
     Tiles t2{};
     if constexpr (BATCH) {
       ++cu.k;
-      more_items = take_item(a, pos, tc, rn, cu);
+      more_items = take_item(a, lanes, pos, tc, rn, cu);
       it2 = cu.it;
       if (more_items) t2 = tiles_of(it2);
     } else {
@@ -597,8 +628,9 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
       for (;;) {
         // the tile after this one: of this item, or the first of the next
         const bool last = !on || ti.jn >= ti.jend;
-        const int bad_n = resources(last ? t2.j : ti.jn, last ? t2.pg[0] : ti.pgn[0],
-                                    last ? t2.pg[1] : ti.pgn[1], last ? (on2 ? it2.end : 0) : it.end, kr, vr);
+        int jn = ti.jn, end = it.end, pg[2] = {ti.pgn[0], ti.pgn[1]};
+        if (last) jn = t2.j, end = on2 ? it2.end : 0, pg[0] = t2.pg[0], pg[1] = t2.pg[1];
+        const int bad_n = resources(jn, pg[0], pg[1], end, kr, vr);
         vmcnt_wait<16>();
         if (merged) lds_barrier();  // every wave has read the merge's slots, which the tiles go to again
         merged = false;
@@ -699,9 +731,19 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
           }
           lds_barrier();
           if (sl >= 0) {
+            // this thread's accumulators: the i-th of each half (128 dims), i0 .. i0 + PER
+            constexpr int PER = MACC / WAVES;
+            const int h = HALVES == 2 ? hf : w >> 1, i0 = HALVES == 2 ? PER * w : PER * (w & 1);
+            const int k0 = HALVES == 2 ? i0 : 8 * h + i0;
+            const u32x4_t from = *reinterpret_cast<const u32x4_t*>(s_slot) + (uint32_t)((k0 * WAVE + lane) * 16);
             const f32x4_t mv = *reinterpret_cast<const f32x4_t*>(s_ml[ct * 16 + c][0]);
             const f32x4_t lv = *reinterpret_cast<const f32x4_t*>(s_ml[ct * 16 + c][1]);
-            const u32x4_t from = *reinterpret_cast<const u32x4_t*>(s_slot) + (uint32_t)(lane * 16);
+            f32x4_t x[WAVES][PER];
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v)
+#pragma unroll
+              for (int k = 0; k < PER; ++k) x[v][k] = *s_acc(from[v], k);
+            __builtin_amdgcn_sched_barrier(0);  // all on their way at once (read one by one: 1.2 us of 2 per merge)
             const float M = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3]));
             float wsc[WAVES], L = 0.f;
 #pragma unroll
@@ -712,20 +754,14 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
             const size_t at = place(ct, sl);
             if (w == 0 && g4 == 0 && hf == 0)
               *reinterpret_cast<float2*>(part_ml + 2 * at) = make_float2(M, L);
-            // this thread's accumulators: the i-th of each half (128 dims), i0 .. i0 + PER
-            constexpr int PER = MACC / WAVES;
-            const int h = HALVES == 2 ? hf : w >> 1, i0 = HALVES == 2 ? PER * w : PER * (w & 1);
-            const int k0 = HALVES == 2 ? i0 : 8 * h + i0;
             f32x4_t mo[PER];
 #pragma unroll
             for (int k = 0; k < PER; ++k) {
               f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int v = 0; v < WAVES; ++v) {
-                const f32x4_t x = *s_acc(from[v] + k0 * (WAVE * 16), k);
+              for (int v = 0; v < WAVES; ++v)
 #pragma unroll
-                for (int ii = 0; ii < 4; ++ii) sum[ii] = __builtin_fmaf(x[ii], wsc[v], sum[ii]);
-              }
+                for (int ii = 0; ii < 4; ++ii) sum[ii] = __builtin_fmaf(x[v][k][ii], wsc[v], sum[ii]);
               mo[k] = sum;
             }
             float* dst = part_o + at * HD + 128 * h + 32 * g4 + i0;
@@ -847,10 +883,33 @@ attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restr
   }
 }
 
-// Least slice of a call: see launch().
-static int least_slice(int B, int Hkv) {
-  const long units = (long)B * Hkv;
-  return units <= 8 ? 32 : units <= 32 ? 128 : 512;
+// How a call is cut, from its sizes alone (not from R: a row's bits are the same in calls of one row).
+struct Plan {
+  int mins, slices;  // least slice; slices that a row can have at most
+  bool batch;
+};
+static Plan plan(int B, int Hkv, int cap, int NS, int window, int sinks) {
+  const auto slices = [&](int ch) {
+    const long dense = ((long)cap + ch - 1) / ch;
+    const long seen = ((long)sinks + ch - 1) / ch + ((long)window + ch - 2) / ch + 1;
+    return (int)std::min<long>(NS, window ? std::min(dense, seen) : dense);
+  };
+  const int cus = compute_units();
+  // An item a workgroup where the workgroups run at once (3 sequences with a window of 500, 32 / 8 heads: slices
+  // of 32 in two rounds 17.3 us, of 64 in one 14.8, in parts 13.7).
+  Plan p{TILE, slices(TILE), false};
+  if ((long)B * Hkv * p.slices <= cus) return p;
+  // Otherwise a third of a CU's share of the positions that the tables hold, 128 to 768: short slices cost
+  // merges (2 us each), long ones balance (an item goes to one workgroup). us per call at least slices of 128 /
+  // 256 / 512 / 768 (the one taken with *): 7 sequences of up to 24,011 positions 50 / 45 / 45 / 45*, 64 of up to
+  // 8,000 154 / 141 / 133 / 133*, 32 with a window of 4,096 120 / 109 / 107 / 103*, 16 of up to 6,000, 4 rows,
+  // 16 / 2 heads, fp8 33 / 30* / 35 / 38.
+  const long span = window ? std::min<long>(cap, (long)window + sinks) : cap;
+  const long share = (long)B * Hkv * span / cus / 3;
+  p.mins = (int)std::min<long>(768, std::max<long>(128, (share + 127) / 128 * 128));
+  p.slices = slices(p.mins);
+  p.batch = true;
+  return p;
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -872,9 +931,11 @@ static hipError_t launch(const void* q, const void* kp, const void* vp, const in
   a.B = B, a.R = R, a.Hq = Hq, a.Hkv = Hkv, a.grp = Hq / Hkv, a.N = N, a.M = M;
   a.lp = __builtin_ctz((unsigned)P);
   a.cap = M * P;
-  a.NS = NS, a.mins = least_slice(B, Hkv);
+  a.NS = NS;
   a.window = window, a.sinks = window ? std::min(sinks, a.cap) : 0;
   a.nd = ns_div(window ? NS - 3 : NS);
+  const Plan pl = plan(B, Hkv, a.cap, NS, window, a.sinks);
+  a.mins = pl.mins;
   a.hch = (a.grp + MAX_COLS - 1) / MAX_COLS;
   a.hc = (a.grp + a.hch - 1) / a.hch;
   const int most = a.hch > 1 ? 1 : std::min(R, MAX_COLS / a.grp), rch = (R + most - 1) / most;
@@ -884,9 +945,8 @@ static hipError_t launch(const void* q, const void* kp, const void* vp, const in
   a.scale_log2 = scale * 1.4426950408889634f, a.v_scale = v_scale;
   // as many workgroups as run at once: 128 KB of LDS each, or 64 KB and 256 registers
   const int NT = a.rc * a.hc <= 16 ? 1 : 2, at_once = compute_units() * (KV8 && NT == 1 ? 2 : 1);
-  const long slices = window ? NS : std::min<long>(NS, (a.cap + a.mins - 1) / a.mins);
-  const bool batch = B * slices * Hkv > 2 * compute_units();
-  a.parts = batch ? std::max(1, at_once / Hkv) : (int)slices;
+  const bool batch = pl.batch;
+  a.parts = batch ? std::max(1, at_once / Hkv) : pl.slices;
   const dim3 grid((unsigned)(a.parts * Hkv), rch * a.hch, batch ? 1 : B), block(WAVES * WAVE);
   const auto* Q = static_cast<const __bf16*>(q);
   const auto *K = static_cast<const char*>(kp), *V = static_cast<const char*>(vp);
