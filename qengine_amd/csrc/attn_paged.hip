@@ -412,7 +412,7 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
   constexpr int SLOT = TILE << LROW;             // LDS bytes of a K tile
   // The merge takes rounds of MACC accumulators of one column tile per wave, through the K slot that the wave's
   // last tile left. An fp8 slot holds half of them; with two column tiles, where registers allow one workgroup
-  // per CU, there is room for buffers of their own (16 sequences of 4 rows, 16 / 2 heads: 38 -> 34 us).
+  // per CU, there is room for buffers of their own (16 sequences of 4 rows, 16 / 2 heads: 4 us of a call).
   constexpr bool OWN = KV8 && NT == 2;
   constexpr int HALVES = KV8 && !OWN ? 2 : 1, MACC = 16 / HALVES;
   static_assert(OWN || MACC * WAVE * 16 == SLOT, "a round of the merge fills a K slot");
@@ -796,9 +796,9 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
 }
 
 // Merge of a row's slices and the gate. A wave takes 256 / G dims of a (head, row): G groups of lanes, lane =
-// (group, 4 dims); a group takes slots s0 + G i + group, and the groups meet in a fixed tree. AHEAD: the first
-// G * U slots are loaded before the position arrives (clamped to the row's slots, those that do not count
-// are selected away): one memory round trip less where the loads are few.
+// (group, 4 dims); a group takes slots s0 + G i + group, and the groups meet in a fixed tree. The first AHEAD * G
+// slots are loaded before the position arrives (clamped to the row's slots, those that do not count are
+// selected away): a memory round trip less for rows of no more slices (64 rows of up to 11: 6.5 -> 6.1 us).
 template <int G>
 __device__ __forceinline__ float groups(float v, bool sum) {
   const auto op = [&](float x, float y) __attribute__((always_inline)) { return sum ? x + y : fmaxf(x, y); };
@@ -810,12 +810,12 @@ __device__ __forceinline__ float groups(float v, bool sum) {
   }
   return v;
 }
-template <int G, bool AHEAD>
+template <int G, int AHEAD>
 __global__ void __launch_bounds__(WAVES * WAVE)
 attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
                           const int* __restrict__ pos, const __bf16* __restrict__ qg,
                           __bf16* __restrict__ out, Call a) {
-  constexpr int U = 4, LD = WAVE / G;  // slots in flight per group, lanes of a group
+  constexpr int LD = WAVE / G;  // lanes of a group
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE, g = lane / LD;
   // waves: (row, head, chunk of dims), the chunk fastest
   const int id = blockIdx.x * WAVES + w, dim = (id % G) * (4 * LD) + 4 * (lane % LD);
@@ -823,40 +823,25 @@ attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restr
   if (row >= a.B * a.R) return;
   const int b = row / a.R, t = row - b * a.R;
   const size_t base = ((size_t)row * a.Hq + h) * a.NS;
-  f32x4_t po[U];
-  float2 ml[U];
-  const auto load = [&](int s0, int n) __attribute__((always_inline)) {
+  f32x4_t O = {0.f, 0.f, 0.f, 0.f};
+  float L = 0.f, M = -INFINITY;
+  const auto load = [&](auto n, int s0, int most, auto& po, auto& ml) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (i > 0 && s0 + G * i >= n) break;  // uniform
-      const int s = min(s0 + G * i + g, n - 1);
+    for (int i = 0; i < decltype(n)::value; ++i) {
+      const int s = min(s0 + G * i + g, most - 1);
       po[i] = *reinterpret_cast<const f32x4_t*>(part_o + (base + s) * HD + dim);
       ml[i] = *reinterpret_cast<const float2*>(part_ml + 2 * (base + s));
     }
   };
+  const auto add = [&](auto n, int s0, int cnt, const auto& po, const auto& ml) __attribute__((always_inline)) {
+    constexpr int U = decltype(n)::value;
+    float mv[U], bm = M;
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    po[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    ml[i] = make_float2(-INFINITY, 0.f);
-  }
-  const __bf16* gp = qg + (size_t)row * a.ldp + (size_t)h * 2 * HD + HD + dim;
-  float gate[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) gate[i] = bf16_to_f32(gp[i]);
-  if constexpr (AHEAD) load(0, a.NS);
-  const int p0 = pos_of(pos, b);
-  if (p0 < 0) return;
-  const int cnt = min(row_slices(a, p0 + t).cnt, a.NS);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) gate[i] = sigmoid_f32(gate[i]);
-  f32x4_t O = {0.f, 0.f, 0.f, 0.f};
-  float L = 0.f, M = -INFINITY;
-  for (int s0 = 0; s0 < cnt; s0 += G * U) {
-    if (!AHEAD || s0 > 0) load(s0, cnt);
-    float mv[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) mv[i] = s0 + G * i + g < cnt ? ml[i].x : -INFINITY;
-    const float bm = groups<G>(fmaxf(M, fmaxf(fmaxf(mv[0], mv[2]), fmaxf(mv[1], mv[3]))), false);
+    for (int i = 0; i < U; ++i) {
+      mv[i] = s0 + G * i + g < cnt ? ml[i].x : -INFINITY;
+      bm = fmaxf(bm, mv[i]);
+    }
+    bm = groups<G>(bm, false);
     if (bm != M) {
       const float r = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - bm);
       O *= r;
@@ -871,6 +856,28 @@ attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restr
       L += (use ? ml[i].y : 0.f) * f;
       O += (use ? po[i] : zero) * f;
     }
+  };
+  using First = std::integral_constant<int, AHEAD>;
+  using More = std::integral_constant<int, 4>;
+  const __bf16* gp = qg + (size_t)row * a.ldp + (size_t)h * 2 * HD + HD + dim;
+  float gate[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) gate[i] = bf16_to_f32(gp[i]);
+  const int p0 = pos_of(pos, b);
+  f32x4_t po[AHEAD];
+  float2 ml[AHEAD];
+  load(First{}, 0, a.NS, po, ml);
+  __builtin_amdgcn_sched_barrier(0);
+  if (p0 < 0) return;
+  const int cnt = min(row_slices(a, p0 + t).cnt, a.NS);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) gate[i] = sigmoid_f32(gate[i]);
+  add(First{}, 0, cnt, po, ml);
+  for (int s0 = G * AHEAD; s0 < cnt; s0 += G * 4) {
+    f32x4_t po[4];
+    float2 ml[4];
+    load(More{}, s0, cnt, po, ml);
+    add(More{}, s0, cnt, po, ml);
   }
   L = groups<G>(L, true);
 #pragma unroll
@@ -972,10 +979,11 @@ static hipError_t launch(const void* q, const void* kp, const void* vp, const in
         <<<dim3((unsigned)((heads * g + WAVES - 1) / WAVES)), block, 0, stream>>>(
             part_o, part_ml, pos, static_cast<const __bf16*>(qg), static_cast<__bf16*>(out), a);
   };
+  // few rows: 16 dims a wave and 64 slots ahead; a batch's: 64 dims, 8 slots
   if (batch)
-    merge(std::integral_constant<int, 4>{}, std::false_type{});
+    merge(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
   else
-    merge(std::integral_constant<int, 16>{}, std::true_type{});
+    merge(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
   return hipGetLastError();
 }
 
