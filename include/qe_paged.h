@@ -37,12 +37,12 @@ extern "C" {
  * j >= p + 1 - window. out = bf16(softmax(q.k * scale) . v * sigmoid(gate)), rounded once, the gate
  * being qg[row][h][256:512]; a row that attends nothing is 0. Key and value rows that a row does not
  * attend do not reach it, whatever they hold (NaN, infinities).
- * Two launches: partials of slices of the cache, merged by the second. A row's slices depend on
- * its own position, on the window and on NS and B alone, so that a row's bits are the same whichever
- * other rows and sequences the call holds.
+ * Two launches: partials of slices of the cache, merged by the second. A row's slices depend on its own
+ * position, on B, Hkv, M * P, NS, window and sinks, and on the device's compute units, so that a row's bits
+ * are the same whatever R is and whichever other rows and sequences the call holds.
  * q rows are contiguous ([B*R][Hq*256], 16-byte aligned), qg rows ldp apart, out rows ldo apart;
- * part_o fp32 [>= B*R][Hq][NS][256] (16-byte aligned) and part_ml fp32 [>= B*R][Hq][NS][2] are the
- * caller's scratch: calls that may overlap need a pair each. NS >= 1, with a window NS >= 4;
+ * part_o fp32 [>= B*R*Hq*NS*256] (16-byte aligned) and part_ml fp32 [>= B*R*Hq*NS*2] are the
+ * caller's scratch (in an order of the kernels' own): calls that may overlap need a pair each. NS >= 1, with a window NS >= 4;
  * 0 <= window < 2^23, sinks >= 0 (ignored without a window). */
 hipError_t qe_attn_decode_paged(const void* q, const void* kp, const void* vp, const int* table,
                                 long ldt, const int* pos, const void* qg, long ldp, float* part_o,

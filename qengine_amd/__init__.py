@@ -91,6 +91,21 @@ def default_splits(max_len: int, hkv: int = 4, cus: int | None = None, kv8: bool
     return max(1, min(math.ceil(max_len / MIN_SLICE), max(1, per_head)))
 
 
+def default_paged_splits(max_len: int, hkv: int = 4, cus: int | None = None) -> int:
+    """Split count NS (part_o.size(2)) of the paged decode for sequences of up to ``max_len`` positions: one
+    sequence alone fills the compute units with workgroups, slices are never shorter than 32 positions, and a
+    window finds the 4 splits that it needs. A batch is balanced by the call itself and uses what it needs of
+    them (one sequence of 131,072 positions, 16 / 2 heads, fp8, from warm caches: NS 32 / 64 / 128 / 256 56.3 / 34.3 /
+    28.6 / 39.7 us; 24 / 4 heads, bf16: 32 / 52 / 64 / 128 103.4 / 83.5 / 84.7 / 92.3)."""
+    cus = cus or compute_units()
+    return max(4, min(math.ceil(max_len / MIN_SLICE), cus // hkv))
+
+
+def alloc_pages_ws(pages: int, device="cuda"):
+    """Caller-owned workspace of ``kv_pages_fork`` and ``kv_pages_compact`` for a pool of ``pages`` pages."""
+    return torch.empty(2 * pages + 8, dtype=torch.int32, device=device)
+
+
 def alloc_partials(n_rows: int, hq: int, ns: int, device="cuda"):
     """Caller-owned split-KV scratch (part_o, part_ml) for up to ``n_rows`` rows."""
     po = torch.empty(n_rows, hq, ns, HEAD_DIM, dtype=torch.float32, device=device)

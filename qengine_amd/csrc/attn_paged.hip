@@ -1,13 +1,19 @@
 // Gated flash-decoding over a paged KV cache for a batch of sequences, 1..8 rows each, optionally
 // with a sliding window and first tokens that stay visible (include/qe_paged.h).
 //
-// The arithmetic of a tile is the contiguous decode's (attn_decode.hip, attn_tile.hpp): four waves
-// of 32-position tiles, S^T = K Q^T and O^T += V^T P^T on MFMA, K one tile ahead through LDS DMA, V in
-// registers. What differs:
-//  * A tile is two halves of 16 positions with a buffer resource each, whose base comes from the page
-//    table, read a tile ahead. Pages are powers of two >= 16, so no half crosses a page.
-//  * Persistent workgroups take equal parts of the call's work, which each derives from pos: a wave scan over
-//    the sequences' tiles. Work goes by the lengths at hand, not by the longest possible.
+// The arithmetic of a tile is the contiguous decode's (attn_decode.hip, attn_tile.hpp): tiles of 32
+// positions a wave, S^T = K Q^T and O^T += V^T P^T on MFMA, K one tile ahead through LDS DMA, V in
+// registers. It streams the cache: 6 flops a byte at 6 heads a group, so HBM bounds it (64 sequences of up to
+// 8,000 positions, 24 / 4 heads, bf16: 718 MB in 129 us, 5.6 TB/s with both launches; one of 131,072, fp8, 16 / 2
+// heads: 268 MB in 48 us), and short calls its two launches (one sequence of 1,000: 9.5 us). What differs:
+//  * A tile's buffer resources have their base from the page table, read a tile ahead. Pages are powers of two;
+//    with pages of 16 positions a tile is two halves with a resource each.
+//  * In a batch every wave is a worker of its own: persistent waves take equal parts of the call's work, which
+//    each derives from pos (a wave scan over the sequences' tiles), and write a slice's partial without meeting
+//    the others. Work goes by the lengths at hand, not by the longest possible. With four waves a slice and a
+//    merge per slice instead, the waves wait for one another and items are four times as coarse (7 sequences
+//    of up to 24,011 positions 43.9 us against 39.0; 64 of up to 8,000 132.6 / 129.4; 16 of up to 6,000, 4 rows, fp8
+//    29.1 / 25.8; 32 with a window of 4,096 100.3 / 103.2).
 //  * Slices start at multiples of their size and tiles go to waves by their place in the slice, both
 //    counted from position 0. So the rows of a call share a slice whatever their windows, a tile that a
 //    row does not attend is an exact no-op for it, and a row's bits depend on no other row or sequence.
@@ -33,13 +39,14 @@ constexpr int MAX_COLS = 32;  // query columns of a workgroup: two MFMA tiles
 struct Call {
   int B, R, Hq, Hkv, grp, N, M, lp;  // lp: log2 of the page size
   int cap;                           // positions a table row can hold
-  int NS, mins;                      // slots of a row's partials; least slice
+  int NS, mins, most;                // slots of a row's partials; least slice; slices that a row can have
   NsDiv nd;
   int window, sinks;
   int rc, hc, hch;                   // rows and heads of a column chunk, head chunks
-  int parts;                         // workgroups of a KV head
+  int parts;                         // waves, or (few items) workgroups, of a KV head
   uint32_t hkv_m;                    // floor(2^32 / Hkv), or 2^32 - 1
   long ldt, ldp, ldo;
+  size_t rh;                         // rows times heads
   float scale_log2, v_scale;
 };
 
@@ -163,9 +170,9 @@ __device__ __forceinline__ void place_item(const Call& a, int rn, Cursor& c) {
 }
 
 // The items of a batch: a sequence's lie along a line, one after another, each as long as its tiles plus
-// OVER, and the sequences follow one another. Workgroup i of a KV head takes the items that begin in the i-th
+// OVER, and the sequences follow one another. Wave i of a KV head takes the items that begin in the i-th
 // of equal parts of the line. Places count from the part's begin.
-constexpr int OVER = 3;  // what an item costs beside its tiles, in tiles
+constexpr int OVER = 2;  // what an item costs beside its tiles, in tiles
 
 // A sequence's length on the line: a little more than its tiles, and OVER for each item.
 __device__ __forceinline__ int line_of(const Call& a, const SeqItems& q, int p0, int rn) {
@@ -397,25 +404,32 @@ __device__ __forceinline__ void take_odd(Tile<KV8>& b, const f32x4_t (&sacc)[NT]
       }
 }
 
-// part_o [rows][Hq][NS][256] (unnormalised O), part_ml [rows][Hq][NS][2] = (max in log2 units, sum).
-// BATCH: persistent workgroups that take a part of the call's items each. While a wave computes the last tile of
-// an item, K of its first tile of the next one is on its way, and V during the merge of the four waves, so
-// that the memory latency of an item's begin is paid once per workgroup. Otherwise (few items) a workgroup is
-// an item: (slice, KV head; sequence), without the search for it.
+// Place of a partial's dims in its 256 floats: [half][ii][i / 4][g4][i % 4] for dim 128 half + 32 g4 + 8 ii + i, so
+// that a store of the accumulators' lanes (c, g4) writes 64 bytes on end, not 16 in each of four lines.
+__device__ __forceinline__ int dim_of(int at) {  // of the first of 4 floats
+  return (at & 128) + 32 * (at >> 2 & 3) + 8 * (at >> 5 & 3) + 4 * (at >> 4 & 1);
+}
+
+// part_o [NS][rows][Hq][256] (unnormalised O, dim_of), part_ml [NS][rows][Hq][2] = (max in log2 units, sum).
+// BATCH: persistent waves that take a part of the call's items each. While a wave computes the last tile of an
+// item, K of its first tile of the next one is on its way, and V while it stores the partial, so that the
+// memory latency of an item's begin is paid once. Otherwise (few items) four waves are a workgroup and an
+// item is (slice, KV head; sequence), without the search for it.
 template <int NT, bool KV8, bool P16, bool BATCH>
 __global__ void __launch_bounds__(WAVES * WAVE) __attribute__((amdgpu_waves_per_eu(NT == 1 && KV8 ? 2 : 1, 2)))
 attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict__ kp,
                            const char* __restrict__ vp, const int* __restrict__ table,
                            const int* __restrict__ pos, float* __restrict__ part_o,
                            float* __restrict__ part_ml, Call a) {
+  constexpr int WPI = BATCH ? 1 : WAVES;         // waves of an item
   constexpr int LROW = KV8 ? 8 : 9;              // log2 of a cache row's bytes
   constexpr int SLOT = TILE << LROW;             // LDS bytes of a K tile
-  // The merge takes rounds of MACC accumulators of one column tile per wave, through the K slot that the wave's
-  // last tile left. An fp8 slot holds half of them; with two column tiles, where registers allow one workgroup
-  // per CU, there is room for buffers of their own (16 sequences of 4 rows, 16 / 2 heads: 4 us of a call).
-  constexpr bool OWN = KV8 && NT == 2;
+  // The merge of four waves takes rounds of MACC accumulators of one column tile per wave, through the K slot that
+  // the wave's last tile left. An fp8 slot holds half of them; with two column tiles, where registers allow one
+  // workgroup per CU, there is room for buffers of their own.
+  constexpr bool OWN = KV8 && NT == 2 && !BATCH;
   constexpr int HALVES = KV8 && !OWN ? 2 : 1, MACC = 16 / HALVES;
-  static_assert(OWN || MACC * WAVE * 16 == SLOT, "a round of the merge fills a K slot");
+  static_assert(BATCH || OWN || MACC * WAVE * 16 == SLOT, "a round of the merge fills a K slot");
   __shared__ __attribute__((aligned(256))) char lds[WAVES * (2 * SLOT + (OWN ? MACC * WAVE * 16 : 0))];
   __shared__ __attribute__((aligned(16))) float s_ml[16 * NT][2][WAVES];  // (m, l) of a column's waves
   __shared__ __attribute__((aligned(16))) uint32_t s_slot[WAVES];
@@ -440,7 +454,7 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
   Lanes lanes{};
   if constexpr (BATCH) {
     lanes = lanes_of(a, pos, tc, rn, lane);
-    if (!first_item(a, lanes, pos, tc, rn, i, a.parts, cu)) return;
+    if (!first_item(a, lanes, pos, tc, rn, i * WAVES + w, a.parts, cu)) return;
   } else {
     const int p = pos_of(pos, blockIdx.z);
     if (p < 0) return;
@@ -478,7 +492,7 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
     int pg[2], pgn[2];
   };
   const auto skip = [&](int j, int jlo) __attribute__((always_inline)) {
-    return j < jlo && j * TILE >= sinks ? j + (jlo - j + WAVES - 1) / WAVES * WAVES : j;
+    return j < jlo && j * TILE >= sinks ? j + (jlo - j + WPI - 1) / WPI * WPI : j;
   };
   const auto pages_of = [&](int (&pg)[2], int b, int j) __attribute__((always_inline)) {
     const int* row = table + (size_t)b * a.ldt;
@@ -490,8 +504,8 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
     Tiles t;
     t.jlo = a.window ? max(it.p0 + it.r0 + 1 - a.window, 0) / TILE : 0;
     t.jend = (it.end + TILE - 1) / TILE;
-    t.j = skip(it.beg / TILE + w, t.jlo);
-    t.jn = skip(t.j + WAVES, t.jlo);
+    t.j = skip(it.beg / TILE + (BATCH ? 0 : w), t.jlo);
+    t.jn = skip(t.j + WPI, t.jlo);
     pages_of(t.pg, it.b, t.j);
     pages_of(t.pgn, it.b, t.jn);
     return t;
@@ -604,7 +618,7 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
       const int p = ti.j * TILE;
       if (!last) {
         ti.j = ti.jn;
-        ti.jn = skip(ti.jn + WAVES, ti.jlo);
+        ti.jn = skip(ti.jn + WPI, ti.jlo);
         pages_of(ti.pgn, it.b, ti.jn);
       }
       if (p + TILE > mk.Lmin || bad || (p < mk.lo_max && p + TILE > mk.sinks)) {
@@ -632,8 +646,6 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
         if (last) jn = t2.j, end = on2 ? it2.end : 0, pg[0] = t2.pg[0], pg[1] = t2.pg[1];
         const int bad_n = resources(jn, pg[0], pg[1], end, kr, vr);
         vmcnt_wait<16>();
-        if (merged) lds_barrier();  // every wave has read the merge's slots, which the tiles go to again
-        merged = false;
         __builtin_amdgcn_sched_barrier(0);
         issue_k<KV8, P16>(nxt, kr, kl);
         __builtin_amdgcn_sched_barrier(0);
@@ -683,33 +695,33 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
     };
     const auto place = [&](int ct, int sl) __attribute__((always_inline)) {
       const int t = trow[ct], head = g * a.grp + hc + (ct * 16 + c - t * hn);
-      return ((size_t)(it.b * a.R + tc + t) * a.Hq + head) * a.NS + sl;
+      return (size_t)sl * a.rh + (size_t)(it.b * a.R + tc + t) * a.Hq + head;
     };
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) l[ct] = group4_sum(l[ct]);
-    merged = it.end - it.beg > TILE;
+    merged = !BATCH && it.end - it.beg > TILE;
     if (!merged) {
-      // one tile: the other waves hold m = -inf, l = 0, O = 0, so that wave 0's are the partial, bit for bit
-      if (w == 0) {
+      // a wave's item; or one tile, where the other waves hold m = -inf, l = 0, O = 0: wave 0's are the partial
+      if (BATCH || w == 0) {
 #pragma unroll
         for (int ct = 0; ct < NT; ++ct) {
           const int sl = slot(ct);
           if (sl < 0) continue;
           const size_t at = place(ct, sl);
           if (g4 == 0) *reinterpret_cast<float2*>(part_ml + 2 * at) = make_float2(m[ct], l[ct]);
-          float* dst = part_o + at * HD + 32 * g4;
+          float* dst = part_o + at * HD + 4 * g4;
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
             for (int ii = 0; ii < 4; ++ii)
 #pragma unroll
               for (int i = 0; i < 8; i += 4)
-                *reinterpret_cast<f32x4_t*>(dst + 128 * hh + 8 * ii + i) =
+                *reinterpret_cast<f32x4_t*>(dst + 128 * hh + 32 * ii + 4 * i) =
                     f32x4_t{acc[ct][8 * hh + i][ii], acc[ct][8 * hh + i + 1][ii], acc[ct][8 * hh + i + 2][ii],
                             acc[ct][8 * hh + i + 3][ii]};
         }
       }
-    } else {
+    } else if constexpr (!BATCH) {
       // the waves' merge, in order 0..3
       const uint32_t park = OWN ? lds_byte_uniform(lds + WAVES * 2 * SLOT + w * (MACC * WAVE * 16)) : cur;
 #pragma unroll
@@ -764,13 +776,13 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
                 for (int ii = 0; ii < 4; ++ii) sum[ii] = __builtin_fmaf(x[v][k][ii], wsc[v], sum[ii]);
               mo[k] = sum;
             }
-            float* dst = part_o + at * HD + 128 * h + 32 * g4 + i0;
+            float* dst = part_o + at * HD + 128 * h + 16 * (i0 >> 2) + 4 * g4 + (i0 & 3);
 #pragma unroll
             for (int ii = 0; ii < 4; ++ii) {
               if constexpr (PER == 4)
-                *reinterpret_cast<f32x4_t*>(dst + 8 * ii) = f32x4_t{mo[0][ii], mo[1][ii], mo[2][ii], mo[3][ii]};
+                *reinterpret_cast<f32x4_t*>(dst + 32 * ii) = f32x4_t{mo[0][ii], mo[1][ii], mo[2][ii], mo[3][ii]};
               else
-                *reinterpret_cast<float2*>(dst + 8 * ii) = make_float2(mo[0][ii], mo[1][ii]);
+                *reinterpret_cast<float2*>(dst + 32 * ii) = make_float2(mo[0][ii], mo[1][ii]);
             }
           }
         }
@@ -797,7 +809,7 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
 
 // Merge of a row's slices and the gate. A wave takes 256 / G dims of a (head, row): G groups of lanes, lane =
 // (group, 4 dims); a group takes slots s0 + G i + group, and the groups meet in a fixed tree. The first AHEAD * G
-// slots are loaded before the position arrives (clamped to the row's slots, those that do not count are
+// slots are loaded before the position arrives (clamped to the slots a row can have; those that do not count are
 // selected away): a memory round trip less for rows of no more slices (64 rows of up to 11: 6.5 -> 6.1 us).
 template <int G>
 __device__ __forceinline__ float groups(float v, bool sum) {
@@ -818,19 +830,20 @@ attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restr
   constexpr int LD = WAVE / G;  // lanes of a group
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE, g = lane / LD;
   // waves: (row, head, chunk of dims), the chunk fastest
-  const int id = blockIdx.x * WAVES + w, dim = (id % G) * (4 * LD) + 4 * (lane % LD);
+  const int id = blockIdx.x * WAVES + w, at = (id % G) * (4 * LD) + 4 * (lane % LD);
+  const int dim = dim_of(at);
   const int rh = id / G, row = (int)((unsigned)rh / (unsigned)a.Hq), h = rh - row * a.Hq;
   if (row >= a.B * a.R) return;
   const int b = row / a.R, t = row - b * a.R;
-  const size_t base = ((size_t)row * a.Hq + h) * a.NS;
+  const size_t base = (size_t)row * a.Hq + h;
   f32x4_t O = {0.f, 0.f, 0.f, 0.f};
   float L = 0.f, M = -INFINITY;
   const auto load = [&](auto n, int s0, int most, auto& po, auto& ml) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < decltype(n)::value; ++i) {
       const int s = min(s0 + G * i + g, most - 1);
-      po[i] = *reinterpret_cast<const f32x4_t*>(part_o + (base + s) * HD + dim);
-      ml[i] = *reinterpret_cast<const float2*>(part_ml + 2 * (base + s));
+      po[i] = *reinterpret_cast<const f32x4_t*>(part_o + ((size_t)s * a.rh + base) * HD + at);
+      ml[i] = *reinterpret_cast<const float2*>(part_ml + 2 * ((size_t)s * a.rh + base));
     }
   };
   const auto add = [&](auto n, int s0, int cnt, const auto& po, const auto& ml) __attribute__((always_inline)) {
@@ -866,7 +879,7 @@ attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restr
   const int p0 = pos_of(pos, b);
   f32x4_t po[AHEAD];
   float2 ml[AHEAD];
-  load(First{}, 0, a.NS, po, ml);
+  load(First{}, 0, a.most, po, ml);
   __builtin_amdgcn_sched_barrier(0);
   if (p0 < 0) return;
   const int cnt = min(row_slices(a, p0 + t).cnt, a.NS);
@@ -902,18 +915,24 @@ static Plan plan(int B, int Hkv, int cap, int NS, int window, int sinks) {
     return (int)std::min<long>(NS, window ? std::min(dense, seen) : dense);
   };
   const int cus = compute_units();
-  // An item a workgroup where the workgroups run at once (3 sequences with a window of 500, 32 / 8 heads: slices
-  // of 32 in two rounds 17.3 us, of 64 in one 14.8, in parts 13.7).
+  // A workgroup an item, slices of 32, where all run at once.
   Plan p{TILE, slices(TILE), false};
   if ((long)B * Hkv * p.slices <= cus) return p;
-  // Otherwise a third of a CU's share of the positions that the tables hold, 128 to 768: short slices cost
-  // merges (2 us each), long ones balance (an item goes to one workgroup). us per call at least slices of 128 /
-  // 256 / 512 / 768 (the one taken with *): 7 sequences of up to 24,011 positions 50 / 45 / 45 / 45*, 64 of up to
-  // 8,000 154 / 141 / 133 / 133*, 32 with a window of 4,096 120 / 109 / 107 / 103*, 16 of up to 6,000, 4 rows,
-  // 16 / 2 heads, fp8 33 / 30* / 35 / 38.
   const long span = window ? std::min<long>(cap, (long)window + sinks) : cap;
-  const long share = (long)B * Hkv * span / cus / 3;
-  p.mins = (int)std::min<long>(768, std::max<long>(128, (share + 127) / 128 * 128));
+  const long work = (long)B * Hkv * span;
+  // Of few sequences with little each, a slice a CU (4 of 16,384 positions, 16 / 2 heads, fp8, as a batch: 24 us,
+  // slices of 256 / 512* / 1,024: 20.0 / 18.7 / 22.5; 3 with a window of 500, 32 / 8 heads, slices of 32 / 64* / 128 /
+  // 256: 16.6 / 13.5 / 13.5 / 15.4).
+  if ((long)B * Hkv <= cus / 8 && work <= 512L * cus) {
+    p.mins = std::max<int>(64, (work / cus + 63) / 64 * 64);
+    p.slices = slices(p.mins);
+    return p;
+  }
+  // Otherwise a batch, slices of about half of a wave's share of the positions that the tables hold: short ones
+  // cost partials (written, read again) and an item's begin each, long ones balance. us at 128 / 256 / 384 / 512 / 768
+  // (* as below): 7 sequences of up to 24,011 positions 46 / 42 / 45 / 39* / 45, 64 of up to 8,000 148 / 138 / 133 /
+  // 129* / 131, 32 with a window of 4,096 115 / 111 / 103* / 113 / 103, 16 of up to 6,000, 4 rows, fp8 26* / 32 / 38.
+  p.mins = (int)std::min<long>(512, std::max<long>(128, (work * 3 / 5 / cus / WAVES + 127) / 128 * 128));
   p.slices = slices(p.mins);
   p.batch = true;
   return p;
@@ -942,34 +961,34 @@ static hipError_t launch(const void* q, const void* kp, const void* vp, const in
   a.window = window, a.sinks = window ? std::min(sinks, a.cap) : 0;
   a.nd = ns_div(window ? NS - 3 : NS);
   const Plan pl = plan(B, Hkv, a.cap, NS, window, a.sinks);
-  a.mins = pl.mins;
+  a.mins = pl.mins, a.most = pl.slices;
   a.hch = (a.grp + MAX_COLS - 1) / MAX_COLS;
   a.hc = (a.grp + a.hch - 1) / a.hch;
   const int most = a.hch > 1 ? 1 : std::min(R, MAX_COLS / a.grp), rch = (R + most - 1) / most;
   a.rc = (R + rch - 1) / rch;
   a.hkv_m = Hkv == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (unsigned)Hkv);
   a.ldt = ldt, a.ldp = ldp, a.ldo = ldo;
+  a.rh = (size_t)B * R * Hq;
   a.scale_log2 = scale * 1.4426950408889634f, a.v_scale = v_scale;
   // as many workgroups as run at once: 128 KB of LDS each, or 64 KB and 256 registers
   const int NT = a.rc * a.hc <= 16 ? 1 : 2, at_once = compute_units() * (KV8 && NT == 1 ? 2 : 1);
   const bool batch = pl.batch;
-  a.parts = batch ? std::max(1, at_once / Hkv) : pl.slices;
-  const dim3 grid((unsigned)(a.parts * Hkv), rch * a.hch, batch ? 1 : B), block(WAVES * WAVE);
+  const int groups = batch ? std::max(1, at_once / Hkv) : pl.slices;
+  a.parts = batch ? groups * WAVES : groups;
+  const dim3 grid((unsigned)(groups * Hkv), rch * a.hch, batch ? 1 : B), block(WAVES * WAVE);
   const auto* Q = static_cast<const __bf16*>(q);
   const auto *K = static_cast<const char*>(kp), *V = static_cast<const char*>(vp);
   const auto go = [&](auto nt, auto p16, auto bt) {
     attn_paged_partials_kernel<decltype(nt)::value, KV8, decltype(p16)::value, decltype(bt)::value>
         <<<grid, block, 0, stream>>>(Q, K, V, table, pos, part_o, part_ml, a);
   };
-  using One = std::integral_constant<int, 1>;
-  using Two = std::integral_constant<int, 2>;
-  const auto by_page = [&](auto nt, auto bt) {
-    P == 16 ? go(nt, std::true_type{}, bt) : go(nt, std::false_type{}, bt);
+  const auto by_batch = [&](auto nt, auto p16) {
+    batch ? go(nt, p16, std::true_type{}) : go(nt, p16, std::false_type{});
   };
-  const auto by_batch = [&](auto nt) {
-    batch ? by_page(nt, std::true_type{}) : by_page(nt, std::false_type{});
+  const auto by_page = [&](auto nt) {
+    P == 16 ? by_batch(nt, std::true_type{}) : by_batch(nt, std::false_type{});
   };
-  NT == 1 ? by_batch(One{}) : by_batch(Two{});
+  NT == 1 ? by_page(std::integral_constant<int, 1>{}) : by_page(std::integral_constant<int, 2>{});
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const long heads = (long)B * R * Hq;

@@ -12,12 +12,16 @@ bit-identical results; on gfx950 up to 0.7 us faster per layer-call for one row 
 8k positions, up to 1.2 us slower for two rows and at 16k, where the fused kernel's single-slot
 KV tile loop costs more than the launch it saves). It allocates only at construction, so a pass
 can be captured in a hipGraph.
+
+PagedCache and PagedGatedAttention are the same for a batch of sequences over one paged cache: a pass
+extends the tables once, then every layer issues attn_prep_paged and attn_decode_paged. The reference
+serves one sequence and has no counterpart.
 """
 from __future__ import annotations
 
 import torch
 
-from . import _C, alloc_partials, default_splits
+from . import _C, alloc_pages_ws, alloc_partials, default_paged_splits, default_splits
 
 HEAD_DIM = 256
 
@@ -63,4 +67,89 @@ class GatedAttention:
         else:
             _C.attn_prep(*prep)
             _C.attn_decode(q, self.kc, self.vc, pos, qg, self.part_o, self.part_ml, out)
+        return out
+
+
+class PagedCache:
+    """The paged KV cache of `layers` layers for up to `sequences` sequences of up to `max_len` positions: pools
+    kp / vp [layers, pages, Hkv, page_size, 256] (bf16, or E4M3FN codes with kv8), one table and its page counts
+    for all layers. What `extend`, `free`, `fork` and `compact` change is device memory of fixed addresses, so a
+    pass that calls them can be captured. Their arguments are int32 device tensors; none allocates or syncs."""
+
+    def __init__(self, hkv: int, max_len: int, sequences: int, pages: int, page_size: int = 64, layers: int = 1,
+                 kv8: bool = False, k_scale: float = 1.0, v_scale: float = 1.0, device="cuda"):
+        if page_size < 16 or page_size > 32768 or page_size & (page_size - 1):
+            raise ValueError("page_size must be a power of two, 16..32768")
+        self.hkv, self.page_size, self.sequences, self.layers = hkv, page_size, sequences, layers
+        self.kv8, self.k_scale, self.v_scale = kv8, k_scale, v_scale
+        width = -(-max_len // page_size)  # entries of a sequence
+        self.max_len = width * page_size
+        dtype = torch.float8_e4m3fn if kv8 else torch.bfloat16
+        shape = (layers, pages, hkv, page_size, HEAD_DIM)
+        self.kp, self.vp = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+        self.table = torch.full((sequences, width), -1, dtype=torch.int32, device=device)
+        self.ref = torch.zeros(pages, dtype=torch.int32, device=device)
+        # of the last extend or fork: pages that it could not give
+        self.missing = torch.zeros(1, dtype=torch.int32, device=device)
+        self.ws = alloc_pages_ws(pages, device)
+
+    def extend(self, pos: torch.Tensor, count: torch.Tensor) -> None:
+        """Maps the pages of positions [pos[b], pos[b] + count[b]) of every sequence b with pos[b] >= 0."""
+        _C.kv_pages_extend(self.table, self.ref, pos, count, self.page_size, self.missing)
+
+    def free(self, first: torch.Tensor, last: torch.Tensor) -> None:
+        """Releases the pages wholly inside [first[b], last[b]) of every sequence b."""
+        _C.kv_pages_free(self.table, self.ref, first, last, self.page_size)
+
+    def fork(self, src: torch.Tensor, dst: torch.Tensor, length: torch.Tensor) -> None:
+        """Sequence dst[i] becomes a copy of the first length[i] positions of src[i]: whole pages are shared, the
+        last partial one is copied. New rows go behind `length`, so neither writes into a shared page."""
+        _C.kv_pages_fork(self.table, self.ref, src, dst, length, self.kp, self.vp, self.missing, self.ws)
+
+    def compact(self) -> None:
+        """Moves the pages in use to the pools' front."""
+        _C.kv_pages_compact(self.table, self.ref, self.kp, self.vp, self.ws)
+
+
+class PagedGatedAttention:
+    """One gated full-attention layer over a PagedCache: the decode-path calls for up to n_max rows per sequence,
+    optionally with a sliding window and first tokens that stay visible. `share`: another layer of the same
+    sizes whose scratch (q, part_o, part_ml) this one uses too, for layers that run one after another."""
+
+    def __init__(self, cache: PagedCache, layer: int, hq: int, q_norm: torch.Tensor, k_norm: torch.Tensor,
+                 rope_theta: float = 1e7, rotary_dim: int = 64, eps: float = 1e-6, n_max: int = 1,
+                 window: int = 0, sinks: int = 0, splits: int | None = None,
+                 share: "PagedGatedAttention | None" = None):
+        d, dev = HEAD_DIM, cache.kp.device
+        self.cache, self.kp, self.vp = cache, cache.kp[layer], cache.vp[layer]
+        self.hq, self.hkv, self.eps, self.window, self.sinks = hq, cache.hkv, eps, window, sinks
+        self.q_norm, self.k_norm = q_norm.to(dev), k_norm.to(dev)
+        self.inv_freq = rope_inv_freq(rope_theta, rotary_dim, dev)
+        if share is not None:
+            self.q, self.part_o, self.part_ml = share.q, share.part_o, share.part_ml
+        else:
+            rows = cache.sequences * n_max
+            self.q = torch.zeros(rows, hq * d, dtype=torch.bfloat16, device=dev)
+            ns = splits or default_paged_splits(cache.max_len, cache.hkv)
+            self.part_o, self.part_ml = alloc_partials(rows, hq, ns, dev)
+        self.q0 = hq * 2 * d
+        self.k1 = self.q0 + cache.hkv * d
+        self.width = self.k1 + cache.hkv * d
+
+    def __call__(self, proj: torch.Tensor, pos: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+        """proj: [sequences * R, >= width] bf16 projection rows (any row stride), R per sequence; pos: int32
+        [sequences], the position of each sequence's first row, negative for an idle one; out: [sequences * R,
+        Hq*256] bf16 rows. Writes K/V of the rows into their pages (mapped by cache.extend) and the gated
+        attention output of each row into out; an idle sequence's rows are left as they are."""
+        pr = proj[:, : self.width]
+        qg, k, v = pr[:, : self.q0], pr[:, self.q0: self.k1], pr[:, self.k1:]
+        q, c = self.q[: proj.shape[0]], self.cache
+        prep = (qg, k, v, self.q_norm, self.k_norm, self.inv_freq, pos, q, self.kp, self.vp, c.table, self.eps)
+        decode = (q, self.kp, self.vp, c.table, pos, qg, self.part_o, self.part_ml, out)
+        if c.kv8:
+            _C.attn_prep_paged_fp8(*prep, c.k_scale, c.v_scale)
+            _C.attn_decode_paged_fp8(*decode, c.k_scale, c.v_scale, self.window, self.sinks)
+        else:
+            _C.attn_prep_paged(*prep)
+            _C.attn_decode_paged(*decode, self.window, self.sinks)
         return out

@@ -227,3 +227,21 @@ def test_capi_pages_reject(capi):
     for kw in (dict(src=None), dict(dst=None), dict(m=0), dict(m=65536), dict(kp=None), dict(N=0)):
         assert lib.qe_kv_pages_copy(*{**copy, **kw}.values(), None) == INVALID, kw
     assert lib.qe_kv_pages_ws_size(5) == 72 and lib.qe_kv_pages_ws_size(0) == 0
+
+
+def test_cache_helpers(native):
+    """Sizes of the host-side helpers, and the cache's refusals (built on the CPU)."""
+    import qengine_amd as qe
+    from qengine_amd.layer import PagedCache
+    assert qe.default_paged_splits(131072, 4, cus=256) == 64
+    assert qe.default_paged_splits(1000, 4, cus=256) == 32
+    assert qe.default_paged_splits(16, 4, cus=256) == 4
+    assert qe.default_paged_splits(131072, 500, cus=256) == 4
+    assert qe.alloc_pages_ws(100, device="cpu").numel() == 208
+    c = PagedCache(2, 100, 3, 7, page_size=32, layers=2, device="cpu")
+    assert c.kp.shape == c.vp.shape == (2, 7, 2, 32, 256) and c.kp.dtype == torch.bfloat16
+    assert c.table.shape == (3, 4) and (c.table == -1).all() and c.max_len == 128 and not c.ref.any()
+    assert PagedCache(1, 16, 1, 1, 16, kv8=True, device="cpu").kp.dtype == torch.float8_e4m3fn
+    for bad in (0, 8, 48, 65536):
+        with pytest.raises(ValueError, match="power of two"):
+            PagedCache(2, 100, 3, 7, page_size=bad, device="cpu")
