@@ -96,6 +96,8 @@ size_t qe_kv_pages_ws_size(int N);
  * into a page of its own. Pages that src does not have, dst does not get. A pair is refused (it changes
  * nothing and counts in missing) if src or dst is not a sequence of the table, or dst is also a source or
  * the dst of another pair. missing[0]: partial pages for which none was free, plus refused pairs.
+ * Neither sequence may write below length afterwards (its pages there are shared): to go back further, fork to
+ * the earlier length.
  * kp / vp: `layers` pools of N pages of page_bytes (a multiple of 16) each, one after another.
  * 1 <= m <= 1024. */
 hipError_t qe_kv_pages_fork(int* table, long ldt, int* ref, const int* src, const int* dst,

@@ -25,6 +25,10 @@ Parity status per function (each is pinned by checks in ``tests/test_oracle.py``
                                                          functions, HF's chunked delta rule, the
                                                          fp64 matrix form, numpy convolution,
                                                          closed forms, rollback invariants)
+  paged_oracle: decode, prep, extend, free, fork, compact
+                                                      -> pinned (the contiguous oracle over gathered
+                                                         pages, brute force, closed forms;
+                                                         tests/test_paged_oracle.py)
 """
 from .attn_oracle import *  # noqa: F401,F403
 from .gemv_oracle import gemv_bf16_ref, gemv_bound, gemv_exact  # noqa: F401

@@ -5,7 +5,8 @@
 // of a row. The cos / sin of the row's rd/2 frequencies, its most expensive step, are computed once per
 // workgroup into LDS, one frequency per thread, while the head's row is on its way; the rotate-half partner
 // goes through the half-wave's own LDS row. A call is a chain of latencies (position, page, row, sincos),
-// not bytes.
+// not bytes: one row, 24 / 4 heads, 4.0 us in a graph, 2.7 of them the kernel; four rows of each of 64 sequences
+// into fp8 pages (7.9 MB) 5.5 us.
 #include "qe_device.hpp"
 #include "qe_paged.h"
 

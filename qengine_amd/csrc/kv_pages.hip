@@ -4,7 +4,9 @@
 // (which page goes to whom) is decided by one workgroup: ranks by ballots, free pages by a scan of ref that
 // stops when enough are found. Everything else (releasing, sharing, renaming entries, moving data) is
 // order-free and spread over the card; the counts are atomics whose sum does not depend on their order.
-// Data moves in 32 KB pieces, eight 16-byte loads in flight per thread.
+// Data moves in 32 KB pieces, eight 16-byte loads in flight per thread, at 5.0 TB/s read and written (a copy of
+// 1 GiB: 5.2). Compacting 500 pages (524 MB) takes 118 us, a fork of eight sequences in 8 layers (33.6 MB) 22, and
+// free, free, extend between two steps of 200 sequences 11.5: one launch each, bound by their chains of loads.
 #include <algorithm>
 #include <type_traits>
 
@@ -17,7 +19,8 @@ namespace pages {
 constexpr int PT = 1024;            // threads of the deciding workgroup
 constexpr int PW = PT / WAVE;
 // Refs per thread and scan step: few in the first one, which nearly always finds what a call needs (a step of 16
-// everywhere: extend 8.1 us against 3.2, compact's plan 8.1 against 2.4, since a compute unit runs all 16 waves of it), more in those after it.
+// everywhere: extend 8.1 us against 3.2, compact's plan 8.1 against 2.4, since one compute unit runs all 16 waves
+// of it), more in those after it.
 constexpr int FEW = 2, MANY = 16;
 constexpr int WS_HEAD = 8;          // workspace: [0] pairs to move; from WS_HEAD on their pages
 

@@ -103,7 +103,8 @@ class PagedCache:
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor, length: torch.Tensor) -> None:
         """Sequence dst[i] becomes a copy of the first length[i] positions of src[i]: whole pages are shared, the
-        last partial one is copied. New rows go behind `length`, so neither writes into a shared page."""
+        last partial one is copied. Both go on at `length` or behind it, where neither writes into a
+        shared page; to go back further, fork to the earlier length."""
         _C.kv_pages_fork(self.table, self.ref, src, dst, length, self.kp, self.vp, self.missing, self.ws)
 
     def compact(self) -> None:
