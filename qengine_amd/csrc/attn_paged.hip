@@ -863,8 +863,9 @@ attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restr
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const bool use = mv[i] != -INFINITY;
-      const float f = use ? __builtin_amdgcn_exp2f(mv[i] - M) : 0.f;
+      // A slot without a finite maximum holds zeros, or NaN from a NaN among the scores, which stays one
+      const bool use = s0 + G * i + g < cnt;
+      const float f = mv[i] != -INFINITY ? __builtin_amdgcn_exp2f(mv[i] - M) : 1.f;
       const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
       L += (use ? ml[i].y : 0.f) * f;
       O += (use ? po[i] : zero) * f;

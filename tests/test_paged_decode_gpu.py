@@ -122,6 +122,22 @@ def test_a_later_rows_values_do_not_reach_an_earlier_row(native, kv, hq, window)
 
 
 @pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("lens", [[0, 40, 700], [0, 3, 700, 1500] + [200] * 30])
+def test_nan_is_not_lost(native, lens, kv):
+    """A row whose query is NaN, or whose attended keys all are, is NaN (no score is a maximum then), and no other
+    row of the call changes."""
+    c = Batch(31, lens, R=2, hq=8, hkv=2, kv=kv)
+    want = Call(c).run(native).view(-1, c.hq, D).clone()
+    c.q.view(-1, c.hq, D)[5, 3, 17] = float("nan")                # row 1 of sequence 2
+    c.kp.view(torch.uint8)[int(c.table[0, 0])] = 0xff             # every key that sequence 0 attends
+    got = Call(c).run(native).view(-1, c.hq, D)
+    assert got[:2].isnan().all() and got[5, 3].isnan().all()
+    rest = torch.ones(got.shape[:2], dtype=torch.bool, device=DEV)
+    rest[:2], rest[5, 3] = False, False
+    assert torch.equal(got[rest], want[rest])
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
 def test_unmapped_and_foreign_pages_are_not_attended(native, kv):
     c = Batch(11, [50, 200, 64, 33], R=2, hq=6, hkv=1, P=16, kv=kv)
     c.table[0, 1] = -1
