@@ -920,20 +920,28 @@ static Plan plan(int B, int Hkv, int cap, int NS, int window, int sinks) {
   Plan p{TILE, slices(TILE), false};
   if ((long)B * Hkv * p.slices <= cus) return p;
   const long span = window ? std::min<long>(cap, (long)window + sinks) : cap;
-  const long work = (long)B * Hkv * span;
-  // Of few sequences with little each, a slice a CU (4 of 16,384 positions, 16 / 2 heads, fp8, as a batch: 24 us,
-  // slices of 256 / 512* / 1,024: 20.0 / 18.7 / 22.5; 3 with a window of 500, 32 / 8 heads, slices of 32 / 64* / 128 /
-  // 256: 16.6 / 13.5 / 13.5 / 15.4).
-  if ((long)B * Hkv <= cus / 8 && work <= 512L * cus) {
-    p.mins = std::max<int>(64, (work / cus + 63) / 64 * 64);
+  const long pairs = (long)B * Hkv, work = pairs * span;
+  const auto least = [&](long share, int most) {
+    return (int)std::min<long>(most, std::max<long>(128, (share + 127) / 128 * 128));
+  };
+  // Slices of a CU's share, up to two a CU: as a batch they would leave most waves without work (us, so / as a batch;
+  // 24 / 4 heads, bf16 if not said): 3 with a window of 500, 32 / 8 heads 11.6 / 13.5, 4 of 16,384, 16 / 2 heads, fp8
+  // 18.7 / 24, 27 of 350, fp8 13.7 / 16.3, 16 of up to 6,000, 4 rows, 16 / 2 heads, fp8 25.0 / 25.9.
+  p.mins = least(work / cus, 512);
+  p.slices = slices(p.mins);
+  if (pairs * p.slices <= 2 * cus) return p;
+  // Few long sequences, where NS makes the slices longer than a batch's: a wave alone would take as long as the
+  // call (5 of up to 96,486, fp8 60.8 / 82; 3 of up to 117,989 92.9 / 108).
+  if (span >= 512L * NS && pairs * NS <= 8 * cus) {
+    p.mins = 256;
     p.slices = slices(p.mins);
     return p;
   }
-  // Otherwise a batch, slices of about half of a wave's share of the positions that the tables hold: short ones
-  // cost partials (written, read again) and an item's begin each, long ones balance. us at 128 / 256 / 384 / 512 / 768
-  // (* as below): 7 sequences of up to 24,011 positions 46 / 42 / 45 / 39* / 45, 64 of up to 8,000 148 / 138 / 133 /
-  // 129* / 131, 32 with a window of 4,096 115 / 111 / 103* / 113 / 103, 16 of up to 6,000, 4 rows, fp8 26* / 32 / 38.
-  p.mins = (int)std::min<long>(512, std::max<long>(128, (work * 3 / 5 / cus / WAVES + 127) / 128 * 128));
+  // A batch, slices of about half of a wave's share of the positions that the tables hold: short ones cost
+  // partials (written, read again) and an item's begin each, long ones balance. us at 128 / 256 / 384 / 512 / 768
+  // (* as below): 7 of up to 24,011 46 / 42 / 45 / 39* / 45, 64 of up to 8,000 148 / 138 / 133 / 129* / 131, 32 with a
+  // window of 4,096 115 / 111 / 103* / 113 / 103, 43 of 3 rows with one of 654, fp8 41* / 45 / - / 56.
+  p.mins = least(work * 3 / 5 / cus / WAVES, 512);
   p.slices = slices(p.mins);
   p.batch = true;
   return p;
@@ -999,11 +1007,14 @@ static hipError_t launch(const void* q, const void* kp, const void* vp, const in
         <<<dim3((unsigned)((heads * g + WAVES - 1) / WAVES)), block, 0, stream>>>(
             part_o, part_ml, pos, static_cast<const __bf16*>(qg), static_cast<__bf16*>(out), a);
   };
-  // few rows: 16 dims a wave and 64 slots ahead; a batch's: 64 dims, 8 slots
-  if (batch)
-    merge(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
-  else
+  // Many slots of few heads: 16 dims a wave and 64 slots ahead, four times the waves (one row of 24 heads, 32 / 64
+  // slots: 9.7 / 51.2 us a call against 10.0 / 52.9). Otherwise 64 dims and 8 slots (37 rows of 24 heads, one slot: 10.2
+  // against 17.5; 6 rows of 32 heads, 6 slots: 11.5 against 13.6).
+  // (not by R: the two add in different orders)
+  if (a.most > 8 && (long)B * Hq <= 64)
     merge(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+  else
+    merge(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
   return hipGetLastError();
 }
 
