@@ -810,12 +810,14 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
 // Merge of a row's slices and the gate. A wave takes 256 / G dims of a (head, row): G groups of lanes, lane =
 // (group, 4 dims); a group takes slots s0 + G i + group, and the groups meet in a fixed tree. The first AHEAD * G
 // slots are loaded before the position arrives (clamped to the slots a row can have; those that do not count are
-// selected away): a memory round trip less for rows of no more slices (64 rows of up to 11: 6.5 -> 6.1 us).
+// selected away): a memory round trip less for rows of no more slices.
 template <int G>
 __device__ __forceinline__ float groups(float v, bool sum) {
   const auto op = [&](float x, float y) __attribute__((always_inline)) { return sum ? x + y : fmaxf(x, y); };
-  v = xor32_pair(v, sum);
-  v = xor16_pair(v, sum);
+  if constexpr (G > 1) {
+    v = xor32_pair(v, sum);
+    v = xor16_pair(v, sum);
+  }
   if constexpr (G == 16) {
     v = op(v, dpp<0x128>(v));               // lane ^ 8
     v = op(v, dpp<0x1B>(dpp<0x141>(v)));    // lane ^ 4
@@ -1007,12 +1009,15 @@ static hipError_t launch(const void* q, const void* kp, const void* vp, const in
         <<<dim3((unsigned)((heads * g + WAVES - 1) / WAVES)), block, 0, stream>>>(
             part_o, part_ml, pos, static_cast<const __bf16*>(qg), static_cast<__bf16*>(out), a);
   };
-  // Many slots of few heads: 16 dims a wave and 64 slots ahead, four times the waves (one row of 24 heads, 32 / 64
-  // slots: 9.7 / 51.2 us a call against 10.0 / 52.9). Otherwise 64 dims and 8 slots (37 rows of 24 heads, one slot: 10.2
-  // against 17.5; 6 rows of 32 heads, 6 slots: 11.5 against 13.6).
-  // (not by R: the two add in different orders)
-  if (a.most > 8 && (long)B * Hq <= 64)
+  // (Not by R: the forms add in different orders.) Many slots of few heads: 16 dims a wave and 64 slots ahead (one
+  // row of 24 heads, 32 / 64 slots: 9.7 / 51.2 us a call against 10.0 / 52.9 with 64 dims and 8 slots). Few slots, or many
+  // heads: all dims a wave and 4 slots (192 rows of 32 heads, one slot: 15.0 against 23.9; 66 of 16, 5 slots: 25.5 / 26.7; 64
+  // of 24, up to 16 slots: 128.8 / 129.7; but 7 of 24, 47 slots: 43.7 / 39.5).
+  const long row = (long)B * Hq;
+  if (a.most > 8 && row <= 64)
     merge(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+  else if (a.most <= 4 || (a.most <= 16 && row >= 256))
+    merge(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
   else
     merge(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
   return hipGetLastError();
