@@ -4,8 +4,8 @@
 // The arithmetic of a tile is the contiguous decode's (attn_decode.hip, attn_tile.hpp): tiles of 32
 // positions a wave, S^T = K Q^T and O^T += V^T P^T on MFMA, K one tile ahead through LDS DMA, V in
 // registers. It streams the cache: 6 flops a byte at 6 heads a group, so HBM bounds it (64 sequences of up to
-// 8,000 positions, 24 / 4 heads, bf16: 718 MB in 129 us, 5.6 TB/s with both launches; one of 131,072, fp8, 16 / 2
-// heads: 268 MB in 48 us), and short calls its two launches (one sequence of 1,000: 9.5 us). What differs:
+// 8,000 positions, 24 / 4 heads, bf16: 718 MB in 128 us, 5.6 TB/s with both launches; one of
+// 131,000, fp8: 268 MB in 49 us), and short calls its two launches (one sequence of 1,000: 9.1 us). What differs:
 //  * A tile's buffer resources have their base from the page table, read a tile ahead. Pages are powers of two;
 //    with pages of 16 positions a tile is two halves with a resource each.
 //  * In a batch every wave is a worker of its own: persistent waves take equal parts of the call's work, which

@@ -306,3 +306,27 @@ def test_two_calls_at_once(native):
             b.run(native)
         torch.cuda.synchronize()
         assert torch.equal(a.out, want[0]) and torch.equal(b.out, want[1])
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (20, 0), (20, 5), (200, 3)])
+@pytest.mark.parametrize("hq,hkv,R,P,M", [(24, 4, 1, 16, 1), (24, 4, 6, 32, 1), (16, 2, 8, 64, 2), (40, 1, 3, 16, 16),
+                                          (6, 3, 2, 128, 2)])
+def test_short_tables(native, hq, hkv, R, P, M, window, sinks, kv):
+    """Short tables, whose rows are one or a few slices, and rows past their end; the same bits where the output's rows
+    are not aligned to 16 bytes."""
+    cap = P * M
+    lens = sorted({0, 1, 7, cap // 2, cap - 1, cap + 3, -1, max(cap - R, 0), cap + 500, 3 * cap})
+    c = Batch(77, [min(n, cap - 1) for n in lens], R=R, hq=hq, hkv=hkv, P=P, kv=kv, window=window, sinks=sinks,
+              trim=False, extra_m=0)
+    c.table, c.M = c.table[:, :M].contiguous(), M
+    c.pos = lens
+    call = Call(c)
+    call.check(native)
+    first = call.out.clone()
+    call.po.fill_(float("nan"))
+    wide = torch.full((c.B * R, hq * D + 8), 7.0, dtype=BF, device=DEV)
+    call.out = wide[:, 4:4 + hq * D]
+    call.run(native)
+    assert torch.equal(call.out, first)
+    assert (wide[:, :4] == 7).all() and (wide[:, 4 + hq * D:] == 7).all()
