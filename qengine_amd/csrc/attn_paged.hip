@@ -12,14 +12,14 @@
 //    each derives from pos (a wave scan over the sequences' tiles), and write a slice's partial without meeting
 //    the others. Work goes by the lengths at hand, not by the longest possible. With four waves a slice and a
 //    merge per slice instead, the waves wait for one another and items are four times as coarse (7 sequences
-//    of up to 24,011 positions 43.9 us against 39.0; 64 of up to 8,000 132.6 / 129.4; 16 of up to 6,000, 4 rows, fp8
-//    29.1 / 25.8; 32 with a window of 4,096 100.3 / 103.2).
+//    of up to 24,011 positions 43.9 us against 39.0; 64 of up to 8,000 132.6 / 129.4; 32 with a window of 4,096
+//    100.3 / 103.2).
 //  * Slices start at multiples of their size and tiles go to waves by their place in the slice, both
 //    counted from position 0. So the rows of a call share a slice whatever their windows, a tile that a
 //    row does not attend is an exact no-op for it, and a row's bits depend on no other row or sequence.
 //  * Masked tiles (a row's end, the edges of a window, unmapped pages): scores outside are -inf, V rows
-//    that no row attends are zeroed, and where a V row that only some rows attend is not finite the
-//    product is formed row by row (0 * inf would reach the others).
+//    that no row attends are zeroed, and a V value that only some rows attend and that is not finite is
+//    taken apart (take_odd; 0 * inf would reach the others).
 //  * The output is rounded once: bf16(O / L * sigmoid(gate)) in fp32 (the contiguous decode keeps the
 //    rounding points of the reference, which has no paged cache).
 #include <algorithm>
