@@ -949,6 +949,12 @@ static Plan plan(int B, int Hkv, int cap, int NS, int window, int sinks) {
   return p;
 }
 
+// plan() as the tests ask for it: the least slice, the slices that a row can have at most, whether it is a batch.
+void decode_form(int B, int Hkv, int cap, int NS, int window, int sinks, int (&form)[3]) {
+  const Plan p = plan(B, Hkv, cap, NS, window, sinks);
+  form[0] = p.mins, form[1] = p.slices, form[2] = p.batch;
+}
+
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <bool KV8>

@@ -5,6 +5,12 @@
 #include "bindings_util.hpp"
 #include "qe_paged.h"
 
+namespace qe {
+namespace paged {
+void decode_form(int B, int Hkv, int cap, int NS, int window, int sinks, int (&form)[3]);  // attn_paged.hip
+}
+}  // namespace qe
+
 namespace {
 
 void same_device(const torch::Tensor& t, std::initializer_list<const torch::Tensor*> others) {
@@ -348,6 +354,13 @@ void bind_paged(py::module_& m) {
           return std::vector<int64_t>{a.t.B, a.R, a.Hq, a.p.Hkv, a.p.N, a.p.P, a.t.M, a.NS, a.t.ld, a.ldp,
                                       a.ldo};
         });
+  // how the decode cuts a call (host only): (least slice, most slices of a row, persistent waves)
+  m.def("_attn_decode_paged_form", [](int B, int Hkv, int cap, int NS, int window, int sinks) {
+    TORCH_CHECK(B >= 1 && Hkv >= 1 && cap >= 1 && NS >= 1 && window >= 0 && sinks >= 0, "sizes must be positive");
+    int f[3];
+    qe::paged::decode_form(B, Hkv, cap, NS, window, window ? std::min(sinks, cap) : 0, f);
+    return std::make_tuple(f[0], f[1], f[2] != 0);
+  });
   m.def("_check_attn_prep_paged",
         [](torch::Tensor qg, torch::Tensor k, torch::Tensor v, torch::Tensor qnw, torch::Tensor knw,
            torch::Tensor inv_freq, torch::Tensor pos, torch::Tensor q_out, torch::Tensor kp,
