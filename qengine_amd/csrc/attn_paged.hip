@@ -19,7 +19,8 @@
 //    row does not attend is an exact no-op for it, and a row's bits depend on no other row or sequence.
 //  * Masked tiles (a row's end, the edges of a window, unmapped pages): scores outside are -inf, V rows
 //    that no row attends are zeroed, and a V value that only some rows attend and that is not finite is
-//    taken apart (take_odd; 0 * inf would reach the others).
+//    taken apart (take_odd; 0 * inf would reach the others). What an attended value of that kind makes of
+//    the output is decided by the merge (odd_values).
 //  * The output is rounded once: bf16(O / L * sigmoid(gate)) in fp32 (the contiguous decode keeps the
 //    rounding points of the reference, which has no paged cache).
 #include <algorithm>
@@ -326,18 +327,21 @@ struct Masks {
 };
 
 // The masks of a tile: scores outside are -inf, V rows that no row attends are 0. True where a V row that
-// some of the rows attend is not finite. bad: halves without a page.
+// some of the rows attend is not finite. bad: halves without a page. in: bit e where the column attends.
 template <int NT, bool KV8>
 __device__ __forceinline__ bool mask_tile(Tile<KV8>& b, f32x4_t (&sacc)[NT][2], int p0, int bad,
-                                          const Masks<NT>& mk, int g4) {
+                                          const Masks<NT>& mk, int g4, uint32_t (&in)[NT]) {
   uint32_t odd = 0;
+#pragma unroll
+  for (int ct = 0; ct < NT; ++ct) in[ct] = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int p = p0 + 16 * (e >> 2) + 4 * g4 + (e & 3);
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) {
-      const bool in = p < mk.L[ct] && (p < mk.sinks || p >= mk.lo[ct]) && !(bad >> (e >> 2) & 1);
-      sacc[ct][e >> 2][e & 3] = in ? sacc[ct][e >> 2][e & 3] : -INFINITY;
+      const bool on = p < mk.L[ct] && (p < mk.sinks || p >= mk.lo[ct]) && !(bad >> (e >> 2) & 1);
+      sacc[ct][e >> 2][e & 3] = on ? sacc[ct][e >> 2][e & 3] : -INFINITY;
+      in[ct] |= on ? 1u << e : 0u;
     }
     const bool any = p < mk.Lmax && (p < mk.sinks || p >= mk.lo_min);
 #pragma unroll
@@ -353,21 +357,20 @@ __device__ __forceinline__ bool mask_tile(Tile<KV8>& b, f32x4_t (&sacc)[NT][2], 
 }
 
 // A masked tile with V values that are not finite, and rows that do not all attend them: 0 * inf in O^T +=
-// V^T P^T would reach the rows that do not. The columns that attend such a value get it here, by an MFMA that
-// counts +inf, -inf and NaN (weights 1, 64, 4096; a tile has 32 positions), and its place in V becomes 0.
+// V^T P^T would reach the rows that do not. The columns that attend such a value get a NaN here, as an unmasked
+// tile's product gives them, by an MFMA that counts these values, and its place in V becomes 0.
 template <int NT, bool KV8>
-__device__ __forceinline__ void take_odd(Tile<KV8>& b, const f32x4_t (&sacc)[NT][2],
-                                         f32x4_t (&acc)[NT][16]) {
+__device__ __forceinline__ void take_odd(Tile<KV8>& b, uint32_t (&bits)[NT], f32x4_t (&acc)[NT][16]) {
   u32x4_t in[NT];  // 1 where the column attends the position
 #pragma unroll
-  for (int ct = 0; ct < NT; ++ct)
+  for (int ct = 0; ct < NT; ++ct) {
+    asm volatile("" : "+v"(bits[ct]));  // (as bits: kept as comparisons they would cost scalar registers)
 #pragma unroll
     for (int d = 0; d < 4; ++d)
-      in[ct][d] = (sacc[ct][d >> 1][2 * (d & 1)] != -INFINITY ? 0x3f80u : 0u) |
-                  (sacc[ct][d >> 1][2 * (d & 1) + 1] != -INFINITY ? 0x3f800000u : 0u);
-  const auto kind = [](uint32_t h) __attribute__((always_inline)) {  // a bf16 in the upper half
-    const uint32_t m = h & 0x7fff0000u;
-    return m < 0x7f800000u ? 0u : m > 0x7f800000u ? 0x4580u : h >> 31 ? 0x4280u : 0x3f80u;
+      in[ct][d] = (bits[ct] >> (2 * d) & 1 ? 0x3f80u : 0u) | (bits[ct] >> (2 * d + 1) & 1 ? 0x3f800000u : 0u);
+  }
+  const auto odd = [](uint32_t h) __attribute__((always_inline)) {  // a bf16 in the upper half
+    return (h & 0x7fff0000u) < 0x7f800000u ? 0u : 0x3f80u;
   };
 #pragma unroll
   for (int hh = 0; hh < 2; ++hh)
@@ -377,19 +380,13 @@ __device__ __forceinline__ void take_odd(Tile<KV8>& b, const f32x4_t (&sacc)[NT]
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
         const uint32_t x = v_bf16(b.v[2 * d][hh])[i >> 1], y = v_bf16(b.v[2 * d + 1][hh])[i >> 1];
-        a[d] = kind(i & 1 ? x & 0xffff0000u : x << 16) | kind(i & 1 ? y & 0xffff0000u : y << 16) << 16;
+        a[d] = odd(i & 1 ? x : x << 16) | odd(i & 1 ? y : y << 16) << 16;
       }
 #pragma unroll
       for (int ct = 0; ct < NT; ++ct) {
         const f32x4_t n = mfma16x16x32(as_bf16x8(a), as_bf16x8(in[ct]), f32x4_t{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int z = (int)n[k];
-          float v = z & 63 ? INFINITY : 0.f;
-          if (z & 0xfc0) v -= INFINITY;  // (inf - inf: NaN)
-          if (z >= 4096) v = __builtin_nanf("");
-          acc[ct][8 * hh + i][k] += v;
-        }
+        for (int k = 0; k < 4; ++k) acc[ct][8 * hh + i][k] = n[k] > 0.f ? __builtin_nanf("") : acc[ct][8 * hh + i][k];
       }
     }
 #pragma unroll
@@ -622,7 +619,8 @@ attn_paged_partials_kernel(const __bf16* __restrict__ q, const char* __restrict_
         pages_of(ti.pgn, it.b, ti.jn);
       }
       if (p + TILE > mk.Lmin || bad || (p < mk.lo_max && p + TILE > mk.sinks)) {
-        if (mask_tile<NT, KV8>(buf, sacc, p, bad, mk, g4)) take_odd<NT, KV8>(buf, sacc, acc);
+        uint32_t in[NT];
+        if (mask_tile<NT, KV8>(buf, sacc, p, bad, mk, g4, in)) take_odd<NT, KV8>(buf, in, acc);
       }
       u32x4_t pb_hi[NT], pb_lo[NT];
       const int none[NT] = {};
@@ -824,13 +822,42 @@ __device__ __forceinline__ float groups(float v, bool sum) {
   }
   return v;
 }
+
+// Which V values that are not finite the row at position p attends in the lane's 4 dims: per dim 3 bits, +inf, -inf,
+// NaN. The groups take positions in turn. bf16 pools.
+template <int G>
+__device__ __forceinline__ uint32_t odd_values(const Call& a, const __bf16* vp, const int* row, int p, int kvh, int dim,
+                                               int g) {
+  uint32_t seen = 0;
+  const auto look = [&](int from, int to) __attribute__((always_inline)) {
+    for (int j = from + g; j < to; j += G) {
+      const int page = row[j >> a.lp];
+      if ((unsigned)page >= (unsigned)a.N) continue;
+      const size_t at = (((size_t)page * a.Hkv + kvh) << a.lp) + (j & ((1 << a.lp) - 1));
+      const u32x2_t v = *reinterpret_cast<const u32x2_t*>(vp + at * HD + dim);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t x = v[i >> 1] >> (16 * (i & 1)) & 0xffffu, m = x & 0x7fffu;
+        seen |= (m < 0x7f80u ? 0u : m > 0x7f80u ? 4u : x >> 15 ? 2u : 1u) << (3 * i);
+      }
+    }
+  };
+  const int L = min(p + 1, a.cap), lo = a.window ? max(p + 1 - a.window, 0) : 0, first = a.window ? min(a.sinks, L) : 0;
+  look(0, first);
+  look(max(lo, first), L);
+#pragma unroll
+  for (int o = WAVE / G; o < WAVE; o <<= 1) seen |= __shfl_xor((int)seen, o);
+  return seen;
+}
+
 template <int G, int AHEAD>
 __global__ void __launch_bounds__(WAVES * WAVE)
 attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
                           const int* __restrict__ pos, const __bf16* __restrict__ qg,
-                          __bf16* __restrict__ out, Call a) {
+                          __bf16* __restrict__ out, const __bf16* __restrict__ vp, const int* __restrict__ table,
+                          Call a) {
   constexpr int LD = WAVE / G;  // lanes of a group
-  const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE, g = lane / LD;
+  const int lane = threadIdx.x & (WAVE - 1), w = uni(threadIdx.x / WAVE), g = lane / LD;
   // waves: (row, head, chunk of dims), the chunk fastest
   const int id = blockIdx.x * WAVES + w, at = (id % G) * (4 * LD) + 4 * (lane % LD);
   const int dim = dim_of(at);
@@ -884,8 +911,9 @@ attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restr
   float2 ml[AHEAD];
   load(First{}, 0, a.most, po, ml);
   __builtin_amdgcn_sched_barrier(0);
-  if (p0 < 0) return;
-  const int cnt = min(row_slices(a, p0 + t).cnt, a.NS);
+  // (An idle row stores nothing. It does not leave here: the loads would move behind the wait for its position.)
+  const int p = p0 < 0 ? 0 : p0 + t;
+  const int cnt = min(row_slices(a, p).cnt, a.NS);
 #pragma unroll
   for (int i = 0; i < 4; ++i) gate[i] = sigmoid_f32(gate[i]);
   add(First{}, 0, cnt, po, ml);
@@ -898,7 +926,20 @@ attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restr
   L = groups<G>(L, true);
 #pragma unroll
   for (int i = 0; i < 4; ++i) O[i] = groups<G>(O[i], true);
-  if (g == 0) {
+  // A V value that is not finite leaves its dim of O not finite, but not with its sign (a weight's two terms and
+  // weights of 0 make NaN of infinities): what the row attends decides. (vp: bf16 pools; E4M3FN has only NaN.)
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) odd |= !(fabsf(O[i]) < INFINITY);
+  if (__builtin_expect(vp && p0 >= 0 && L < INFINITY && __any(odd), 0)) {
+    const uint32_t seen = odd_values<G>(a, vp, table + (size_t)b * a.ldt, p, h / a.grp, dim, g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t s = seen >> (3 * i) & 7;
+      if (s) O[i] = s == 1 ? INFINITY : s == 2 ? -INFINITY : __builtin_nanf("");
+    }
+  }
+  if (g == 0 && p0 >= 0) {
     __bf16* op = out + (size_t)row * a.ldo + (size_t)h * HD + dim;
 #pragma unroll
     for (int i = 0; i < 4; ++i)  // a row that attends nothing: 0
@@ -1013,7 +1054,8 @@ static hipError_t launch(const void* q, const void* kp, const void* vp, const in
     constexpr int g = decltype(G)::value;
     attn_paged_combine_kernel<g, decltype(ahead)::value>
         <<<dim3((unsigned)((heads * g + WAVES - 1) / WAVES)), block, 0, stream>>>(
-            part_o, part_ml, pos, static_cast<const __bf16*>(qg), static_cast<__bf16*>(out), a);
+            part_o, part_ml, pos, static_cast<const __bf16*>(qg), static_cast<__bf16*>(out),
+            KV8 ? nullptr : static_cast<const __bf16*>(vp), table, a);
   };
   // (Not by R: the forms add in different orders.) Many slots of few heads: 16 dims a wave and 64 slots ahead (one
   // row of 24 heads, 32 / 64 slots: 9.7 / 51.2 us a call against 10.0 / 52.9 with 64 dims and 8 slots). Few slots, or many
