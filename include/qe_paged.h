@@ -37,7 +37,8 @@ extern "C" {
  * j >= p + 1 - window. out = bf16(softmax(q.k * scale) . v * sigmoid(gate)), rounded once, the gate
  * being qg[row][h][256:512]; a row that attends nothing is 0. Key and value rows that a row does not
  * attend do not reach it, whatever they hold (NaN, infinities). A dim of V in which a row attends +inf, -inf,
- * or both or a NaN, is +inf, -inf, or NaN before the gate, whatever the weights of those positions.
+ * or both or a NaN, is +inf, -inf, or NaN before the gate, whatever the weights of those positions. A row whose
+ * attended scores all are -inf, or of which one is NaN or +inf, is NaN.
  * Two launches: partials of slices of the cache, merged by the second. A row's slices depend on its own
  * position, on B, Hkv, M * P, NS, window and sinks, and on the device's compute units, so that a row's bits
  * are the same whatever R is and whichever other rows and sequences the call holds.

@@ -823,11 +823,22 @@ __device__ __forceinline__ float groups(float v, bool sum) {
   return v;
 }
 
-// Which V values that are not finite the row at position p attends in the lane's 4 dims: per dim 3 bits, +inf, -inf,
-// NaN. The groups take positions in turn. bf16 pools.
+// The positions that the row at position p attends where they have a page: [0, first) and [lo, L).
+struct Reach {
+  int first, lo, L;
+};
+__device__ __forceinline__ Reach reach_of(const Call& a, int p) {
+  Reach r;
+  r.L = min(p + 1, a.cap);
+  r.first = a.window ? min(a.sinks, r.L) : 0;
+  r.lo = max(a.window ? max(p + 1 - a.window, 0) : 0, r.first);
+  return r;
+}
+// Which V values that are not finite the row attends in the lane's 4 dims: per dim 3 bits, +inf, -inf, NaN. The groups
+// take positions in turn. bf16 pools.
 template <int G>
-__device__ __forceinline__ uint32_t odd_values(const Call& a, const __bf16* vp, const int* row, int p, int kvh, int dim,
-                                               int g) {
+__device__ __forceinline__ uint32_t odd_values(const Call& a, const __bf16* vp, const int* row, const Reach& r, int kvh,
+                                               int dim, int g) {
   uint32_t seen = 0;
   const auto look = [&](int from, int to) __attribute__((always_inline)) {
     for (int j = from + g; j < to; j += G) {
@@ -842,12 +853,22 @@ __device__ __forceinline__ uint32_t odd_values(const Call& a, const __bf16* vp, 
       }
     }
   };
-  const int L = min(p + 1, a.cap), lo = a.window ? max(p + 1 - a.window, 0) : 0, first = a.window ? min(a.sinks, L) : 0;
-  look(0, first);
-  look(max(lo, first), L);
+  look(0, r.first);
+  look(r.lo, r.L);
 #pragma unroll
   for (int o = WAVE / G; o < WAVE; o <<= 1) seen |= __shfl_xor((int)seen, o);
   return seen;
+}
+// Whether the row attends any position.
+__device__ __forceinline__ bool attends_any(const Call& a, const int* row, const Reach& r, int lane) {
+  bool any = false;
+  const auto look = [&](int from, int to) __attribute__((always_inline)) {
+    if (from >= to) return;
+    for (int j = (from >> a.lp) + lane; j <= (to - 1) >> a.lp; j += WAVE) any |= (unsigned)row[j] < (unsigned)a.N;
+  };
+  look(0, r.first);
+  look(r.lo, r.L);
+  return __any(any);
 }
 
 template <int G, int AHEAD>
@@ -932,13 +953,16 @@ attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restr
 #pragma unroll
   for (int i = 0; i < 4; ++i) odd |= !(fabsf(O[i]) < INFINITY);
   if (__builtin_expect(vp && p0 >= 0 && L < INFINITY && __any(odd), 0)) {
-    const uint32_t seen = odd_values<G>(a, vp, table + (size_t)b * a.ldt, p, h / a.grp, dim, g);
+    const uint32_t seen = odd_values<G>(a, vp, table + (size_t)b * a.ldt, reach_of(a, p), h / a.grp, dim, g);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t s = seen >> (3 * i) & 7;
       if (s) O[i] = s == 1 ? INFINITY : s == 2 ? -INFINITY : __builtin_nanf("");
     }
   }
+  // No weight at all: the row attends nothing, or every score is -inf, which has no softmax.
+  if (__builtin_expect(L == 0.f && p0 >= 0 && attends_any(a, table + (size_t)b * a.ldt, reach_of(a, p), lane), 0))
+    L = __builtin_nanf("");
   if (g == 0 && p0 >= 0) {
     __bf16* op = out + (size_t)row * a.ldo + (size_t)h * HD + dim;
 #pragma unroll

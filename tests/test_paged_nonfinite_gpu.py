@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+import paged_exact
 from paged_cases import BF, D
 from paged_exact import Big
 from test_paged_decode_gpu import DEV, Call
@@ -81,3 +82,38 @@ def test_attended_values_that_are_not_finite(native, form, kv):
     for t in range(R):
         c.R, c.q, c.qg, c.pos = 1, q[:, t].contiguous(), qg[:, t].contiguous(), [n + t for n in lens]
         assert same(Call(c).run(native).view(c.B, c.hq, D), want[:, t]), t
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_scores_of_minus_infinity(native, form):
+    """A row whose attended scores all are -inf has no softmax: NaN, not the 0 of a row that attends nothing. Beside finite
+    scores they weigh nothing. One score of +inf: NaN."""
+    c = make(form, "bf16")
+    c.q.view(-1, c.hq, D)[..., 0].abs_().clamp_(min=0.25)
+    clean = Call(c).run(native).view(c.B, c.R, c.hq, D).clone()
+    for b, n in enumerate(c.pos):
+        # every third sequence: all keys up to row 0's, every second one of them, none; the next: no page at all
+        for j in range(0, n + 1, 1 + b % 3) if b % 3 < 2 else ():
+            c.kp[int(c.table[b, j // c.P]), :, j % c.P, 0] = -INF
+    if c.B > 5:
+        c.table[5] = -1
+        c.kp[int(c.table[8, c.pos[8] // c.P]), :, c.pos[8] % c.P, 0] = INF
+    k = Call(c)
+    got = k.run(native).view_as(clean)
+    want, _ = paged_exact.decode(c, k.kp, k.vp, k.table, k.q, k.qg)
+    want = want.view_as(clean)
+    for b, n in enumerate(c.pos):
+        for t in range(c.R):
+            if c.B > 5 and b == 5:
+                assert (got[b, t] == 0).all()
+            elif c.B > 5 and b == 8:
+                assert got[b, t].isnan().all()
+            elif b % 3 == 2:
+                assert same(got[b, t], clean[b, t]), (b, t)
+            elif all(j <= n for j in range(n + t + 1) if attends(c, n + t, j)) and b % 3 == 0:
+                assert got[b, t].isnan().all(), (b, t)
+            else:
+                # sum |q k| / 16 of a finite score is below 20 (256 products of unit normals: 163 / 16 on average, its
+                # deviation 0.8), so weights are off by 2 * 262 * 2^-24 * 20 + 2^-15 < 2^-10, times |V| < 6; then one rounding
+                tol = 6 * 2.0 ** -10 + 2.0 ** -8 * want[b, t].abs()
+                assert ((got[b, t].double() - want[b, t]).abs() <= tol).all(), (b, t)
