@@ -13,8 +13,9 @@
  *   table     int32 [B][M], rows ldt entries apart: the page that holds positions [jP, (j+1)P) of
  *             sequence b. An entry outside [0, N) names no page (-1 by convention)
  *   ref       int32 [N]: table entries that name the page. 0: the page is free
- *   pos       int32 [B]: the position of a sequence's first row. Negative: the sequence is idle, and
- *             no op reads its rows or writes anything for it
+ *   pos       int32 [B]: the position of a sequence's first row. Negative: the sequence is idle: no op
+ *             writes anything for it, and what its rows hold is of no account. The rows have to be
+ *             there all the same: they are loaded before the position is known
  *   rows      row b * R + t of a call is the token of sequence b at position pos[b] + t
  * M * P <= 2^23 - 64 positions per sequence; 1 <= B <= 1024.
  * Every device index (pages, sequences, positions) is checked against these sizes on the device;
