@@ -835,28 +835,41 @@ __device__ __forceinline__ Reach reach_of(const Call& a, int p) {
   return r;
 }
 // Which V values that are not finite the row attends in the lane's 4 dims: per dim 3 bits, +inf, -inf, NaN. The groups
-// take positions in turn. bf16 pools.
+// take positions in turn, U at a time each, until what is sought (the same in every group) is NaN. bf16 pools.
 template <int G>
 __device__ __forceinline__ uint32_t odd_values(const Call& a, const __bf16* vp, const int* row, const Reach& r, int kvh,
-                                               int dim, int g) {
+                                               int dim, int g, const bool (&sought)[4]) {
+  constexpr int U = 4;
   uint32_t seen = 0;
   const auto look = [&](int from, int to) __attribute__((always_inline)) {
-    for (int j = from + g; j < to; j += G) {
-      const int page = row[j >> a.lp];
-      if ((unsigned)page >= (unsigned)a.N) continue;
-      const size_t at = (((size_t)page * a.Hkv + kvh) << a.lp) + (j & ((1 << a.lp) - 1));
-      const u32x2_t v = *reinterpret_cast<const u32x2_t*>(vp + at * HD + dim);
+    for (int j0 = from + g; __any(j0 < to); j0 += G * U) {
+      int page[U];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t x = v[i >> 1] >> (16 * (i & 1)) & 0xffffu, m = x & 0x7fffu;
-        seen |= (m < 0x7f80u ? 0u : m > 0x7f80u ? 4u : x >> 15 ? 2u : 1u) << (3 * i);
+      for (int u = 0; u < U; ++u) page[u] = j0 + G * u < to ? row[(j0 + G * u) >> a.lp] : -1;
+      u32x2_t v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const size_t at = (((size_t)page[u] * a.Hkv + kvh) << a.lp) + ((j0 + G * u) & ((1 << a.lp) - 1));
+        v[u] = u32x2_t{0u, 0u};
+        if ((unsigned)page[u] < (unsigned)a.N) v[u] = *reinterpret_cast<const u32x2_t*>(vp + at * HD + dim);
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x = v[u][i >> 1] >> (16 * (i & 1)) & 0xffffu, m = x & 0x7fffu;
+          seen |= (m < 0x7f80u ? 0u : m > 0x7f80u ? 4u : x >> 15 ? 2u : 1u) << (3 * i);
+        }
+#pragma unroll
+      for (int o = WAVE / G; o < WAVE; o <<= 1) seen |= __shfl_xor((int)seen, o);
+      bool open = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) open |= sought[i] && (seen >> (3 * i) & 7) < 3;  // (3: both infinities; 4: a NaN)
+      if (!__any(open)) return;
     }
   };
   look(0, r.first);
   look(r.lo, r.L);
-#pragma unroll
-  for (int o = WAVE / G; o < WAVE; o <<= 1) seen |= __shfl_xor((int)seen, o);
   return seen;
 }
 // Whether the row attends any position.
@@ -949,14 +962,14 @@ attn_paged_combine_kernel(const float* __restrict__ part_o, const float* __restr
   for (int i = 0; i < 4; ++i) O[i] = groups<G>(O[i], true);
   // A V value that is not finite leaves its dim of O not finite, but not with its sign (a weight's two terms and
   // weights of 0 make NaN of infinities): what the row attends decides. (vp: bf16 pools; E4M3FN has only NaN.)
-  bool odd = false;
+  bool odd[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) odd |= !(fabsf(O[i]) < INFINITY);
-  if (__builtin_expect(vp && p0 >= 0 && L < INFINITY && __any(odd), 0)) {
-    const uint32_t seen = odd_values<G>(a, vp, table + (size_t)b * a.ldt, reach_of(a, p), h / a.grp, dim, g);
+  for (int i = 0; i < 4; ++i) odd[i] = !(fabsf(O[i]) < INFINITY);
+  if (__builtin_expect(vp && p0 >= 0 && L < INFINITY && __any(odd[0] || odd[1] || odd[2] || odd[3]), 0)) {
+    const uint32_t seen = odd_values<G>(a, vp, table + (size_t)b * a.ldt, reach_of(a, p), h / a.grp, dim, g, odd);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t s = seen >> (3 * i) & 7;
+      const uint32_t s = odd[i] ? seen >> (3 * i) & 7 : 0;
       if (s) O[i] = s == 1 ? INFINITY : s == 2 ? -INFINITY : __builtin_nanf("");
     }
   }
