@@ -39,7 +39,8 @@ extern "C" {
  * being qg[row][h][256:512]; a row that attends nothing is 0. Key and value rows that a row does not
  * attend do not reach it, whatever they hold (NaN, infinities). A dim of V in which a row attends +inf, -inf,
  * or both or a NaN, is +inf, -inf, or NaN before the gate, whatever the weights of those positions. A row whose
- * attended scores all are -inf, or of which one is NaN or +inf, is NaN.
+ * attended scores all are -inf, or of which one is NaN or +inf, is NaN. Sums are in fp32: finite values of V
+ * beyond 2^120 / (positions attended) may overflow.
  * Two launches: partials of slices of the cache, merged by the second. A row's slices depend on its own
  * position, on B, Hkv, M * P, NS, window and sinks, and on the device's compute units, so that a row's bits
  * are the same whatever R is and whichever other rows and sequences the call holds.

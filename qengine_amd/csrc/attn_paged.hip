@@ -5,15 +5,18 @@
 // positions a wave, S^T = K Q^T and O^T += V^T P^T on MFMA, K one tile ahead through LDS DMA, V in
 // registers. It streams the cache: 6 flops a byte at 6 heads a group, so HBM bounds it (64 sequences of up to
 // 8,000 positions, 24 / 4 heads, bf16: 718 MB in 128 us, 5.6 TB/s with both launches; one of
-// 131,000, fp8: 268 MB in 49 us), and short calls its two launches (one sequence of 1,000: 9.1 us). What differs:
+// 131,000, fp8: 268 MB in 49 us), and short calls its two launches (one sequence of 1,000: 9.2 us). What differs:
 //  * A tile's buffer resources have their base from the page table, read a tile ahead. Pages are powers of two;
 //    with pages of 16 positions a tile is two halves with a resource each.
 //  * In a batch every wave is a worker of its own: persistent waves take equal parts of the call's work, which
 //    each derives from pos (a wave scan over the sequences' tiles), and write a slice's partial without meeting
-//    the others. Work goes by the lengths at hand, not by the longest possible. With four waves a slice and a
-//    merge per slice instead, the waves wait for one another and items are four times as coarse (7 sequences
+//    the others. The parts go by the lengths at hand; the least slice and the form of the call by what the tables
+//    can hold (plan()), so that short sequences in wide tables are cut coarsely (2 of 1,000, 24 / 4 heads, tables
+//    of 1,024 / 8,192 / 131,072 positions: 9.7 / 12.4 / 17.0 us). With four waves a slice and a merge per slice instead, the waves wait for one another and items are four times as coarse (7 sequences
 //    of up to 24,011 positions 43.9 us against 39.0; 64 of up to 8,000 132.6 / 129.4; 32 with a window of 4,096
 //    100.3 / 103.2).
+//  * Above 32 query columns (rows times heads a group) the rows are cut into chunks, each a pass over the cache
+//    (16 sequences of 4,000, 24 / 4 heads, bf16, 5 / 6 rows: 61.5 / 91.4 us).
 //  * Slices start at multiples of their size and tiles go to waves by their place in the slice, both
 //    counted from position 0. So the rows of a call share a slice whatever their windows, a tile that a
 //    row does not attend is an exact no-op for it, and a row's bits depend on no other row or sequence.
@@ -1095,9 +1098,9 @@ static hipError_t launch(const void* q, const void* kp, const void* vp, const in
             KV8 ? nullptr : static_cast<const __bf16*>(vp), table, a);
   };
   // (Not by R: the forms add in different orders.) Many slots of few heads: 16 dims a wave and 64 slots ahead (one
-  // row of 24 heads, 32 / 64 slots: 9.7 / 51.2 us a call against 10.0 / 52.9 with 64 dims and 8 slots). Few slots, or many
-  // heads: all dims a wave and 4 slots (192 rows of 32 heads, one slot: 15.0 against 23.9; 66 of 16, 5 slots: 25.5 / 26.7; 64
-  // of 24, up to 16 slots: 128.8 / 129.7; but 7 of 24, 47 slots: 43.7 / 39.5).
+  // row of 24 heads, 32 / 64 slots: 10.4 / 51.2 us a call in a graph against 10.6 / 52.8 with 64 dims and 8 slots). Few
+  // slots, or many heads: all dims a wave and 4 slots (192 rows of 32 heads, one slot: 42.4 against 50.7; 66 of 16, 8
+  // slots: 61.9 / 62.3; 64 of 24, up to 16 slots: 127.7 / 128.6; but 7 of 24, 47 slots: 44.7 / 40.4).
   const long row = (long)B * Hq;
   if (a.most > 8 && row <= 64)
     merge(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
