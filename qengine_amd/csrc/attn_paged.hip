@@ -10,11 +10,12 @@
 //    with pages of 16 positions a tile is two halves with a resource each.
 //  * In a batch every wave is a worker of its own: persistent waves take equal parts of the call's work, which
 //    each derives from pos (a wave scan over the sequences' tiles), and write a slice's partial without meeting
-//    the others. The parts go by the lengths at hand; the least slice and the form of the call by what the tables
-//    can hold (plan()), so that short sequences in wide tables are cut coarsely (2 of 1,000, 24 / 4 heads, tables
-//    of 1,024 / 8,192 / 131,072 positions: 9.7 / 12.4 / 17.0 us). With four waves a slice and a merge per slice instead, the waves wait for one another and items are four times as coarse (7 sequences
-//    of up to 24,011 positions 43.9 us against 39.0; 64 of up to 8,000 132.6 / 129.4; 32 with a window of 4,096
-//    100.3 / 103.2).
+//    the others. With four waves a slice and a merge per slice instead, the waves wait for one another and items
+//    are four times as coarse (7 sequences of up to 24,011 positions 43.9 us against 39.0; 64 of up to 8,000
+//    132.6 / 129.4; 32 with a window of 4,096 100.3 / 103.2).
+//  * The parts go by the lengths at hand; the least slice and the form of the call by what the tables can hold
+//    (plan()), so that short sequences in wide tables are cut coarsely (2 of 1,000, 24 / 4 heads, tables of 1,024 /
+//    8,192 / 131,072 positions: 9.7 / 12.4 / 17.0 us).
 //  * Above 32 query columns (rows times heads a group) the rows are cut into chunks, each a pass over the cache
 //    (16 sequences of 4,000, 24 / 4 heads, bf16, 5 / 6 rows: 61.5 / 91.4 us).
 //  * Slices start at multiples of their size and tiles go to waves by their place in the slice, both
