@@ -1,0 +1,69 @@
+/* Linear layers on 4-bit weights for gfx950 (MI355X): weights in microscaled 4-bit floating point ("mx4"), the
+ * 8-bit rows that multiply them ("mx8"), made by a norm with the residual's addition, by SwiGLU or from plain
+ * rows, and the product of the two on the scaled matrix instructions.
+ *
+ * Both formats hold blocks of 32 values along a row (the last one filled up with zeros) under one scale, a power
+ * of two whose code is its exponent + 127. The scale is the smallest 2^e, e in [-127, 127], at which the block's
+ * largest magnitude does not round past the largest code: below 7 for E2M1 (largest 6), at most 464 for E4M3
+ * (largest 448). Codes are value / 2^e rounded to nearest, ties to even. A block that holds an infinity or NaN has
+ * the NaN scale (code 255) and all of its values are NaN.
+ *
+ * Device pointers, element strides; every entry point enqueues on `stream`, allocates nothing, never
+ * synchronises, and returns hipErrorInvalidValue (before any launch) for unsupported arguments. The reference
+ * has no counterpart (its 4-bit weights are integers: csrc/gemv_w4.h:9-55). */
+#ifndef QE_MX_H
+#define QE_MX_H
+
+#include <stddef.h>
+#include <hip/hip_runtime_api.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Limits of every entry point below: rows and N up to 2^24, widths up to 2^20, row strides below 2^23. */
+#define QE_MX_MAX_ROWS (1 << 24)
+#define QE_MX_MAX_WIDTH (1 << 20)
+
+/* Bytes of an [N][K] weight in mx4 (0 if N or K is out of range): tiles of 16 rows by 128 values, in the order in
+ * which a wave's lanes read them, then the scales. 17/32 byte a value where 16 divides N and 512 divides K. */
+size_t qe_mx4_bytes(int N, int K);
+
+/* wq = the mx4 form of w [N][ldw] bf16 (rows K wide). wq: qe_mx4_bytes(N, K) bytes, 16-byte aligned, all of them
+ * written. Valid: N >= 1, K >= 1, ldw >= K. */
+hipError_t qe_mx4_quant(const void* w, long ldw, void* wq, int N, int K, hipStream_t stream);
+
+/* out [N][ldo] bf16 (rows K wide) = the values that wq stands for (exact: each is a bf16 value). */
+hipError_t qe_mx4_dequant(const void* wq, void* out, long ldo, int N, int K, hipStream_t stream);
+
+/* mx8 rows: q [n][ldq] E4M3FN codes, ceil(K / 32) * 32 wide (zeros from K on), s [n][lds] scale codes,
+ * ceil(K / 32) wide. q 16-byte aligned, ldq a multiple of 16. Row r is computed exactly as in a 1-row call.
+ *
+ * qe_quant_mx8: of x [n][ldx] bf16.
+ * qe_swiglu_mx8: of silu(g) * u in fp32, gu [n][ldg] = [g (K) | u (K)] bf16.
+ * qe_rmsnorm1p_mx8: of x * rsqrt(mean(x^2) + eps) * (1 + w) in fp32, w [K] bf16. With delta [n][ldd], x is
+ * bf16(x + delta) and is written to sum [n][ldsum] (sum may be x itself, or delta); without, sum is NULL. */
+hipError_t qe_quant_mx8(const void* x, long ldx, void* q, long ldq, void* s, long lds, int n, int K,
+                        hipStream_t stream);
+hipError_t qe_swiglu_mx8(const void* gu, long ldg, void* q, long ldq, void* s, long lds, int n, int K,
+                         hipStream_t stream);
+hipError_t qe_rmsnorm1p_mx8(const void* x, long ldx, const void* delta, long ldd, const void* w, void* sum,
+                            long ldsum, void* q, long ldq, void* s, long lds, int n, int K, float eps,
+                            hipStream_t stream);
+
+/* out[r][j] = bf16(sum over k of x[r][k] * w[j][k]), x the values of the mx8 rows xq [n][ldx], xs [n][lds] and w
+ * those of wq (mx4 of [N][K]), products and sums in fp32. K is a multiple of 32 (the width of xq). out [n][ldo]
+ * bf16. A NaN of x[r] reaches every out[r][j].
+ * ws: qe_gemm_mx4_ws_size(n, N, K) bytes, 16-byte aligned, any contents, one per call in flight (NULL where that
+ * is 0; with fewer bytes the call runs without it, in another order of sums).
+ * Valid: n >= 1, N >= 1, K >= 32, ldx >= K and a multiple of 16, xq and wq 16-byte aligned, lds >= K / 32,
+ * ldo >= N. */
+hipError_t qe_gemm_mx4(const void* wq, const void* xq, long ldx, const void* xs, long lds, void* out, long ldo,
+                       int n, int N, int K, void* ws, size_t ws_bytes, hipStream_t stream);
+size_t qe_gemm_mx4_ws_size(int n, int N, int K);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* QE_MX_H */

@@ -42,6 +42,7 @@ from ._C import (  # noqa: E402,F401
     commit,
     embed,
     gdn_step_n,
+    gemm_mx4,
     gemv_bf16,
     kv_pages_compact,
     kv_pages_copy,
@@ -50,8 +51,14 @@ from ._C import (  # noqa: E402,F401
     kv_pages_free,
     l2_persist_limit,
     mtp_select,
+    mx4_bytes,
+    mx4_dequant,
+    mx4_quant,
+    mx4_ws_bytes,
     prefill_ws_bytes,
+    quant_mx8,
     rmsnorm1p,
+    rmsnorm1p_mx8,
     set_gdn_early,
     set_gdn_phases,
     set_pdl_launch,
@@ -59,6 +66,7 @@ from ._C import (  # noqa: E402,F401
     split_size,
     stream_window,
     swiglu,
+    swiglu_mx8,
     version,
 )
 
@@ -119,3 +127,22 @@ def alloc_prefill_ws(rows: int, hq: int, hkv: int, max_len: int, device="cuda"):
     a captured call splits the cache as an eager one does, with the same bits."""
     n = prefill_ws_bytes(rows, hq, hkv, max_len)
     return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def alloc_mx4(n_out: int, width: int, device="cuda"):
+    """Buffer of an [n_out, width] weight in microscaled 4-bit floating point, for ``mx4_quant``."""
+    return torch.empty(mx4_bytes(n_out, width), dtype=torch.uint8, device=device)
+
+
+def alloc_mx8(rows: int, width: int, device="cuda"):
+    """Buffers (q, s) of ``rows`` rows in microscaled 8-bit floating point: E4M3 codes, ``width`` rounded up to a
+    multiple of 32, and a scale for every 32 of them."""
+    blocks = -(-width // 32)
+    return (torch.empty(rows, blocks * 32, dtype=torch.float8_e4m3fn, device=device),
+            torch.empty(rows, blocks, dtype=torch.float8_e8m0fnu, device=device))
+
+
+def alloc_mx4_ws(rows: int, n_out: int, width: int, device="cuda"):
+    """Caller-owned workspace of ``gemm_mx4`` for ``rows`` rows (another row count may need more: take the largest),
+    one per call in flight. Calls on fewer rows than it was made for, or without one, are valid too."""
+    return torch.empty(mx4_ws_bytes(rows, n_out, width), dtype=torch.uint8, device=device)

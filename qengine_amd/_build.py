@@ -1,7 +1,7 @@
 """Build recipe for qengine_amd's native code (no setuptools, no hipify).
 
   libqe_attn.so  : gfx950 HIP kernels + the C ABI of include/qe_attn.h, include/qe_gemv.h,
-                   include/qe_step.h, include/qe_gdn.h and include/qe_paged.h (hipcc).
+                   include/qe_step.h, include/qe_gdn.h, include/qe_paged.h and include/qe_mx.h (hipcc).
   _C<ext>.so     : torch extension with the reference's op signatures (g++ against torch's
                    ROCm build), linked to libqe_attn.so through $ORIGIN.
 
@@ -27,7 +27,8 @@ ARCH = "gfx950"
 
 HIP_SOURCES = ["attn_prep.hip", "attn_decode.hip", "attn_combine.hip", "attn_prefill.hip",
                "attn_prefill_wide.hip", "attn_paged.hip", "attn_prep_paged.hip", "kv_pages.hip",
-               "gemv.hip", "gemv_lds.hip", "step.hip", "gdn.hip", "gdn_split.hip"]
+               "gemv.hip", "gemv_lds.hip", "step.hip", "gdn.hip", "gdn_split.hip",
+               "mx_weight.hip", "mx_rows.hip", "mx_gemm.hip"]
 # Per-source code-generation flags. The prefill tile loop keeps 128 fp32 accumulators live; the
 # compiler's default MFMA register form parks them in AGPRs and copies all of them into VGPRs
 # on every iteration. The VGPR form keeps them in place. The max-ILP machine scheduler keeps
@@ -41,7 +42,7 @@ SOURCE_FLAGS = {"attn_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", *MAX_
                 "attn_prefill_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", *MAX_ILP],
                 "attn_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                 "attn_combine.hip": MAX_ILP, "gdn_split.hip": MAX_ILP, "gemv_lds.hip": MAX_ILP}
-BINDINGS = ["bindings", "bindings_paged"]  # .cpp
+BINDINGS = ["bindings", "bindings_paged", "bindings_mx"]  # .cpp
 LIB = PKG / "libqe_attn.so"
 EXT = PKG / ("_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 
@@ -100,7 +101,7 @@ def build_ext() -> Path:
               str(CSRC / (name + ".cpp")), "-o", str(obj)])
         return str(obj)
 
-    with ThreadPoolExecutor(max_workers=2) as ex:
+    with ThreadPoolExecutor(max_workers=3) as ex:
         objs = list(ex.map(compile_one, BINDINGS))
     tmp = EXT.with_suffix(".tmp")
     _run(["g++", "-shared", "-fPIC", *objs, "-o", str(tmp),

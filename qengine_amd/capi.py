@@ -1,5 +1,5 @@
 """ctypes binding of the C ABI in include/qe_attn.h, include/qe_gemv.h, include/qe_step.h,
-include/qe_gdn.h and include/qe_paged.h (libqe_attn.so), without the torch extension.
+include/qe_gdn.h, include/qe_paged.h and include/qe_mx.h (libqe_attn.so), without the torch extension.
 
 This is the binding a non-torch host (or a test that must go through the C ABI) uses. Tensor
 arguments may be torch tensors (their data_ptr is passed) or raw integer device addresses.
@@ -73,6 +73,14 @@ SIGNATURES = {
     "qe_kv_pages_fork": (_I, [_P, _L, _P, _P, _P, _P, _I, _P, _P, _I, _Z, _P, _P, _I, _I, _I, _I, _P]),
     "qe_kv_pages_compact": (_I, [_P, _L, _P, _P, _P, _I, _Z, _P, _I, _I, _I, _P]),
     "qe_kv_pages_copy": (_I, [_P, _P, _I, _Z, _P, _P, _I, _I, _P]),
+    "qe_mx4_bytes": (_Z, [_I, _I]),
+    "qe_mx4_quant": (_I, [_P, _L, _P, _I, _I, _P]),
+    "qe_mx4_dequant": (_I, [_P, _P, _L, _I, _I, _P]),
+    "qe_quant_mx8": (_I, [_P, _L, _P, _L, _P, _L, _I, _I, _P]),
+    "qe_swiglu_mx8": (_I, [_P, _L, _P, _L, _P, _L, _I, _I, _P]),
+    "qe_rmsnorm1p_mx8": (_I, [_P, _L, _P, _L, _P, _P, _L, _P, _L, _P, _L, _I, _I, _F, _P]),
+    "qe_gemm_mx4": (_I, [_P, _P, _L, _P, _L, _P, _L, _I, _I, _I, _P, _Z, _P]),
+    "qe_gemm_mx4_ws_size": (_Z, [_I, _I, _I]),
     "qe_gdn_step_n": (_I, [_P, _P, _P, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I,
                            _I, _F, _P]),
 }

@@ -649,6 +649,7 @@ void gdn_step_n(torch::Tensor qkv, torch::Tensor z, torch::Tensor b, torch::Tens
 }
 
 void bind_paged(py::module_& m);  // bindings_paged.cpp
+void bind_mx(py::module_& m);     // bindings_mx.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "MI355X (gfx950) gated-attention decode ops with qengine._C's signatures";
@@ -774,4 +775,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_gdn_early", [](bool) {},
         "no-op: the reference's overlap-with-producer A/B switch (no dependent launch on HIP)");
   bind_paged(m);
+  bind_mx(m);
 }

@@ -16,12 +16,17 @@ can be captured in a hipGraph.
 PagedCache and PagedGatedAttention are the same for a batch of sequences over one paged cache: a pass
 extends the tables once, then every layer issues attn_prep_paged and attn_decode_paged. The reference
 serves one sequence and has no counterpart.
+
+MX4Linear and MX4MLP are linear layers on 4-bit weights (microscaled E2M1 codes, where the reference's W4Linear has
+integers: python/qengine/engine.py:74-186) for decode rows and prompt chunks alike: MX4MLP is the second half of
+Engine._layer (engine.py:460-466), norm with the residual's addition, gate and up, SwiGLU, down, in four launches.
 """
 from __future__ import annotations
 
 import torch
 
-from . import _C, alloc_pages_ws, alloc_partials, default_paged_splits, default_splits
+from . import (_C, alloc_mx4, alloc_mx4_ws, alloc_mx8, alloc_pages_ws, alloc_partials, default_paged_splits,
+               default_splits)
 
 HEAD_DIM = 256
 
@@ -154,3 +159,49 @@ class PagedGatedAttention:
             _C.attn_prep_paged(*prep)
             _C.attn_decode_paged(*decode, self.window, self.sinks)
         return out
+
+
+class MX4Linear:
+    """y = x W^T with the weight [N, K] held as 4-bit codes with scales, for up to `rows` 8-bit rows. Owns the codes
+    and the product's workspace, both made at construction, so calls can be captured. Calls of one layer, or of
+    layers that `share` a workspace, follow one another."""
+
+    def __init__(self, weight: torch.Tensor, rows: int = 8, share: "MX4Linear | None" = None):
+        self.n_out, self.width, self.rows = weight.shape[0], weight.shape[1], rows
+        dev = weight.device
+        self.wq = alloc_mx4(self.n_out, self.width, dev)
+        _C.mx4_quant(weight, self.wq)
+        need = max(_C.mx4_ws_bytes(n, self.n_out, self.width) for n in range(1, rows + 1))
+        if share is not None and share.ws.numel() >= need:
+            self.ws = share.ws
+        else:
+            self.ws = torch.empty(need, dtype=torch.uint8, device=dev)
+
+    def __call__(self, q: torch.Tensor, s: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+        """q, s: 8-bit rows as `rmsnorm1p_mx8`, `swiglu_mx8` or `quant_mx8` write them; out: [n, N] bf16 rows."""
+        _C.gemm_mx4(self.wq, q, s, out, self.ws)
+        return out
+
+
+class MX4MLP:
+    """One layer's MLP on 4-bit weights for up to `rows` rows: h = bf16(h + delta), then
+    down(silu(gate(x)) * up(x)) of its norm x. gate_up: [2 I, H] (gate rows first), down: [H, I], both bf16."""
+
+    def __init__(self, norm: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, eps: float = 1e-6,
+                 rows: int = 8):
+        dev, H, I = norm.device, down.shape[0], down.shape[1]
+        self.norm, self.eps = norm, eps
+        self.gate_up = MX4Linear(gate_up, rows)
+        self.down = MX4Linear(down, rows, share=self.gate_up)
+        self.x, self.act = alloc_mx8(rows, H, dev), alloc_mx8(rows, I, dev)
+        self.gu = torch.empty(rows, 2 * I, dtype=torch.bfloat16, device=dev)
+
+    def __call__(self, h: torch.Tensor, delta: torch.Tensor | None, out: torch.Tensor) -> torch.Tensor:
+        """h: [n, H] bf16 residual rows, updated in place where there is a delta [n, H]; out: [n, H] bf16 rows
+        (delta itself is fine: it is read before)."""
+        n = h.shape[0]
+        xq, xs, aq, as_, gu = *(t[:n] for t in self.x), *(t[:n] for t in self.act), self.gu[:n]
+        _C.rmsnorm1p_mx8(h, delta, self.norm, xq, xs, self.eps)
+        self.gate_up(xq, xs, gu)
+        _C.swiglu_mx8(gu, aq, as_)
+        return self.down(aq, as_, out)
