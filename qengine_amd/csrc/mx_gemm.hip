@@ -1,6 +1,7 @@
 // The product of 8-bit rows and a 4-bit weight (microscaled formats) on gfx950's scaled matrix instructions: codes
 // and scales go into them as they lie in memory, no value is converted.
 #include "mx_common.hpp"
+#include "mx_gemm.hpp"
 
 namespace qe {
 namespace mx {
@@ -90,6 +91,8 @@ extern "C" hipError_t qe_gemm_mx4(const void* wq, const void* xq, long ldx, cons
   auto* O = static_cast<__bf16*>(out);
   if (n <= 16)
     gemm_mx4_kernel<1><<<dim3(RT), dim3(WAVES * WAVE), 0, stream>>>(W, X, ldx, S, lds, O, ldo, n, N, K);
+  else if (n > 128)
+    return gemm_tiles(W, X, ldx, S, lds, O, ldo, n, N, K, stream);
   else
     gemm_mx4_kernel<4><<<dim3(RT, (n + 63) / 64), dim3(WAVES * WAVE), 0, stream>>>(W, X, ldx, S, lds, O, ldo, n, N, K);
   return hipGetLastError();
