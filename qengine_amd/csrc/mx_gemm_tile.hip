@@ -15,14 +15,15 @@ __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b0, u32x4_t b1, f3
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, d, 4, 0, SA, (int)sa, SB, (int)sb);
 }
 
+// A stage holds 64 values along K of a tile's rows and weight rows.
 template <int WX, int WW, int TX, int TW>
 struct Tile {
   static constexpr int WAVES = WX * WW, ROWS = WX * TX * 32, COLS = WW * TW * 32;
-  static constexpr int XB = ROWS * 128, STAGE = XB + COLS * 64;  // bytes of a stage: x, then the weight
-  static constexpr int DX = (ROWS / 8 + WAVES - 1) / WAVES, DW = (COLS / 16 + WAVES - 1) / WAVES;  // a wave's loads
-  static_assert(WAVES % 2 == 0, "a wave's loads of x are of one parity");
+  static constexpr int XB = ROWS * 64, STAGE = XB + COLS * 32;  // bytes: x, then the weight
+  static constexpr int STAGES = 6;
+  static constexpr int DX = (ROWS / 16 + WAVES - 1) / WAVES, DW = (COLS / 32 + WAVES - 1) / WAVES;  // a wave's loads
   static constexpr int PITCH = TW * 64 + 16;  // of a row in the epilogue, bytes
-  static constexpr int LDS = 3 * STAGE > WAVES * 32 * PITCH ? 3 * STAGE : WAVES * 32 * PITCH;
+  static constexpr int LDS = STAGES * STAGE > WAVES * 32 * PITCH ? STAGES * STAGE : WAVES * 32 * PITCH;
 };
 
 template <int WX, int WW, int TX, int TW>
@@ -41,59 +42,63 @@ gemm_mx4_tile_kernel(const uint8_t* wq, const uint8_t* xq, long ldx, const uint8
   const int x0 = (tile % xtiles) * T::ROWS, c0 = (tile / xtiles) * T::COLS, rt0 = c0 / 16;
   const int KT = L.KT, Kb = K / BLOCK;
 
-  // x: 8 rows of 128 bytes a load; slot c of row i holds chunk c ^ (i / 2 % 8). Rows and chunks past the matrix are zeros.
+  // x: 16 rows of 64 bytes a load; slot c of row i holds chunk c ^ (i / 4 % 4). The weight: half of two 16-row
+  // tiles' 1 KB a load. Rows and chunks past the matrix are zeros.
   const __amdgpu_buffer_rsrc_t xr =
       make_rsrc_uniform(xq + (size_t)x0 * ldx, (uint32_t)((size_t)(min(T::ROWS, n - x0) - 1) * ldx + K));
   const __amdgpu_buffer_rsrc_t wr = make_rsrc_uniform(wq + (size_t)rt0 * KT * 1024,
                                                       (uint32_t)min(T::COLS / 16, L.RT - rt0) * KT * 1024u);
-  const int chunk16 = ((lane & 7) ^ ((w & 1) * 4 + (lane >> 4))) * 16;
+  const int chunk16 = ((lane & 3) ^ (lane >> 4)) * 16;
   uint32_t xo[T::DX], wo[T::DW], xl[T::DX], wl[T::DW];
 #pragma unroll
   for (int i = 0; i < T::DX; ++i) {
-    const int id = min(w + i * T::WAVES, T::ROWS / 8 - 1);
-    xo[i] = (uint32_t)((id * 8 + (lane >> 3)) * ldx + chunk16);
+    const int id = min(w + i * T::WAVES, T::ROWS / 16 - 1);
+    xo[i] = (uint32_t)((id * 16 + (lane >> 2)) * ldx + chunk16);
     xl[i] = lds_byte_uniform(smem) + id * 1024;
   }
 #pragma unroll
   for (int i = 0; i < T::DW; ++i) {
-    const int id = min(w + i * T::WAVES, T::COLS / 16 - 1);
-    wo[i] = (uint32_t)id * KT * 1024u + lane * 16;
+    const int id = min(w + i * T::WAVES, T::COLS / 32 - 1);
+    wo[i] = (uint32_t)(id * 2 + (lane >> 5)) * KT * 1024u + (lane & 31) * 16;
     wl[i] = lds_byte_uniform(smem) + T::XB + id * 1024;
   }
-  auto fetch = [&](int kt, int stage, int i) {  // load i of this wave
-    if (i < T::DX) {
-      const uint32_t past = kt * 128 + chunk16 >= K ? 0x80000000u : 0u;  // outside the buffer
+  constexpr int LOADS = T::DX + T::DW;
+  auto fetch = [&](int t, int slot) {  // this wave's loads of stage t
+    const uint32_t past = t * 64 + chunk16 >= K ? 0x80000000u : 0u;  // outside the buffer
+#pragma unroll
+    for (int i = 0; i < T::DX; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          xr, (__attribute__((address_space(3))) void*)(uintptr_t)(xl[i] + stage * T::STAGE), 16,
-          (int)((xo[i] + kt * 128) | past), 0, 0, 0);
-    } else {
+          xr, (__attribute__((address_space(3))) void*)(uintptr_t)(xl[i] + slot * T::STAGE), 16,
+          (int)((xo[i] + t * 64) | past), 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < T::DW; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          wr, (__attribute__((address_space(3))) void*)(uintptr_t)(wl[i - T::DX] + stage * T::STAGE), 16,
-          (int)(wo[i - T::DX] + min(kt, KT - 1) * 1024), 0, 0, 0);
-    }
+          wr, (__attribute__((address_space(3))) void*)(uintptr_t)(wl[i] + slot * T::STAGE), 16,
+          (int)(wo[i] + min(t, 2 * KT - 1) * 512), 0, 0, 0);
   };
 
   // Scales of four steps: of x, 16 bytes of lane r's row; of the weight, a dword for blocks g and 2 + g of a tile. The
   // last ones of x come from the row's end, shifted down: no byte past the row is read, and blocks past K
   // get code 0.
+  const __amdgpu_buffer_rsrc_t sr = make_rsrc_uniform(wq + L.scales() + (size_t)rt0 * L.KS * 256,
+                                                      (uint32_t)min(T::COLS / 16, L.RT - rt0) * L.KS * 256u);
+  const uint32_t so = (uint32_t)(ww * TW * 2 + (r >> 4)) * L.KS * 256u + ((r & 15) + 16 * g) * 4;
   const uint8_t* xp[TX];
 #pragma unroll
   for (int i = 0; i < TX; ++i) xp[i] = xs + (size_t)min(x0 + (wx * TX + i) * 32 + r, n - 1) * lds;
-  const uint8_t* sp[TW];
-#pragma unroll
-  for (int j = 0; j < TW; ++j)
-    sp[j] = wq + L.scales() + (size_t)min(rt0 + (ww * TW + j) * 2 + (r >> 4), L.RT - 1) * L.KS * 256 +
-            ((r & 15) + 16 * g) * 4;
   uint32_t sw[TW][2], sw2[TW][2];
   u32x4_t sx[TX], sx2[TX];
-  auto scales = [&](int J) {  // J < KS, and at least 16 blocks
+  constexpr int SCALES = 2 * TW + TX;  // loads of scales()
+  auto scales = [&](int J) {  // from K's end on anything: never used
+    const bool more = J < L.KS && Kb >= 16;
 #pragma unroll
     for (int j = 0; j < TW; ++j)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        sw2[j][h] = *reinterpret_cast<const uint32_t*>(sp[j] + (size_t)J * 256 + h * 128);
+        sw2[j][h] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(
+            sr, (int)(so + j * 2 * L.KS * 256 + min(J, L.KS - 1) * 256 + h * 128), 0, 0);
 #pragma unroll
-    for (int i = 0; i < TX; ++i) __builtin_memcpy(&sx2[i], xp[i] + min(J * 16, Kb - 16), 16);
+    for (int i = 0; i < TX; ++i) __builtin_memcpy(&sx2[i], more ? xp[i] + min(J * 16, Kb - 16) : wq, 16);
   };
   auto take = [&](int J) {  // the loaded ones become those of steps 4 J ..
     const int cut = Kb >= 16 ? min(max(J * 16 - (Kb - 16), 0), 16) : 0;  // bytes
@@ -122,29 +127,29 @@ gemm_mx4_tile_kernel(const uint8_t* wq, const uint8_t* xq, long ldx, const uint8
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  const uint8_t* xf = smem + (wx * TX * 32 + r) * 128;
-  const uint8_t* wf = smem + T::XB + (ww * TW * 2 + (r >> 4)) * 1024 + ((r & 15) + 16 * g) * 16;
-  const int slot = r / 2 & 7;
-  u32x4_t a[2][TW], b[2][2];
-  auto read_w = [&](int stage, int h) {
+  const uint8_t* xf = smem + (wx * TX * 32 + r) * 64;
+  const uint8_t* wf = smem + T::XB + (ww * TW * 2 + (r >> 4)) * 512 + ((r & 15) + 16 * g) * 16;
+  const int at0 = (g ^ (r / 4 & 3)) << 4, at1 = ((2 + g) ^ (r / 4 & 3)) << 4;
+  u32x4_t a[TW], b[TX][2];
+  auto read = [&](int slot) {
 #pragma unroll
-    for (int j = 0; j < TW; ++j)
-      a[h][j] = *reinterpret_cast<const u32x4_t*>(wf + stage * T::STAGE + j * 2048 + h * 512);
-  };
-  auto read_x = [&](int stage, int h, int i, int to) {
-    const uint8_t* p = xf + stage * T::STAGE + i * 4096;
-    b[to][0] = *reinterpret_cast<const u32x4_t*>(p + (((4 * h + g) ^ slot) << 4));
-    b[to][1] = *reinterpret_cast<const u32x4_t*>(p + (((4 * h + 2 + g) ^ slot) << 4));
+    for (int j = 0; j < TW; ++j) a[j] = *reinterpret_cast<const u32x4_t*>(wf + slot * T::STAGE + j * 1024);
+#pragma unroll
+    for (int i = 0; i < TX; ++i) {
+      b[i][0] = *reinterpret_cast<const u32x4_t*>(xf + slot * T::STAGE + i * 2048 + at0);
+      b[i][1] = *reinterpret_cast<const u32x4_t*>(xf + slot * T::STAGE + i * 2048 + at1);
+    }
   };
 
-  constexpr int LOADS = T::DX + T::DW, GROUPS = 2 * TX, PER = (LOADS + GROUPS - 1) / GROUPS;
   if (Kb >= 16) {
     scales(0);
   } else {  // one group of four steps: its scales a byte at a time
 #pragma unroll
     for (int j = 0; j < TW; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) sw2[j][h] = *reinterpret_cast<const uint32_t*>(sp[j] + h * 128);
+      for (int h = 0; h < 2; ++h)
+        sw2[j][h] =
+            (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(sr, (int)(so + j * 2 * L.KS * 256 + h * 128), 0, 0);
 #pragma unroll
     for (int i = 0; i < TX; ++i) {
       sx2[i] = u32x4_t{0u, 0u, 0u, 0u};
@@ -156,48 +161,53 @@ gemm_mx4_tile_kernel(const uint8_t* wq, const uint8_t* xq, long ldx, const uint8
     }
   }
 #pragma unroll
-  for (int i = 0; i < LOADS; ++i) fetch(0, 0, i);
-#pragma unroll
-  for (int i = 0; i < LOADS; ++i) fetch(1, 1, i);
-  int stage = 0;
-  // A step, 128 values: its loads have landed once only the next step's are out. The products come in groups of TW;
-  // beside a group's, the next group's operands are read and loads for the step after the next are issued
-  // (all of them ahead of the first products would keep the matrix cores waiting for the load unit).
-#define QE_STEP(S)                                                                                         \
-  {                                                                                                        \
-    const int k = kt + S;                                                                                  \
-    vmcnt_wait<LOADS>();                                                                                   \
-    lds_barrier();                                                                                         \
-    __builtin_amdgcn_sched_barrier(0);                                                                     \
-    read_w(stage, 0);                                                                                      \
-    read_x(stage, 0, 0, 0);                                                                                \
-    __builtin_amdgcn_sched_barrier(0);                                                                     \
-    const int next = stage >= 1 ? stage - 1 : 2;                                                           \
-    _Pragma("unroll") for (int q = 0; q < GROUPS; ++q) {                                                   \
-      const int h = q / TX, i = q % TX;                                                                    \
-      if (q + 1 == TX) read_w(stage, 1);                                                                   \
-      if (q + 1 < GROUPS) read_x(stage, (q + 1) / TX, (q + 1) % TX, (q + 1) & 1);                          \
-      _Pragma("unroll") for (int j = 0; j < TW; ++j) {                                                     \
-        if (j == 1 || TW == 1) {                                                                           \
-          __builtin_amdgcn_sched_barrier(0);                                                               \
-          if (S == 1 && q == 0 && kt + 4 < KT) scales(kt / 4 + 1);                                         \
-          _Pragma("unroll") for (int t = q * PER; t < (q + 1) * PER && t < LOADS; ++t)                     \
-              fetch(k + 2, next, t);                                                                       \
-          __builtin_amdgcn_sched_barrier(0);                                                               \
-        }                                                                                                  \
-        acc[i][j] = h == 0 ? mfma32<S, 0>(a[0][j], b[q & 1][0], b[q & 1][1], acc[i][j], sw[j][0], sx[i][S]) \
-                           : mfma32<S, 2>(a[1][j], b[q & 1][0], b[q & 1][1], acc[i][j], sw[j][1], sx[i][S]); \
-      }                                                                                                    \
-      __builtin_amdgcn_sched_barrier(0);                                                                   \
-    }                                                                                                      \
-    stage = stage == 2 ? 0 : stage + 1;                                                                    \
-    if (k + 1 >= KT) break;                                                                                \
+  for (int t = 0; t < T::STAGES - 1; ++t) fetch(t, t);
+  vmcnt_wait<(T::STAGES - 2) * LOADS>();
+  lds_barrier();
+  // Two halves of the workgroup, a wave of each on every SIMD, take turns: between two barriers one half reads its
+  // operands of a stage and issues loads, the other multiplies, so the matrix cores always have a wave that does
+  // nothing else. The first half reads stage t in turn 2 t, the second in turn 2 t + 1; stage t + 5 goes into
+  // the place of stage t - 1, which both have read by then, and stage t + 1 has landed for every wave before
+  // turn 2 t + 2: only the four after it are out (and, from the third stage of eight, the next scales).
+  const bool second = w >= T::WAVES / 2;
+  int slot = 0;
+  if (second) lds_barrier();
+#define QE_HALF(S, H)                                                                                       \
+  {                                                                                                         \
+    constexpr int OUT = (T::STAGES - 2) * LOADS + (2 * S + H >= 2 && 2 * S + H <= 5 ? SCALES : 0);          \
+    read(slot);                                                                                             \
+    __builtin_amdgcn_sched_barrier(0);                                                                      \
+    if (S == 1 && H == 0) scales(kt / 4 + 1);                                                               \
+    __builtin_amdgcn_sched_barrier(0);                                                                      \
+    fetch(2 * (kt + S) + H + T::STAGES - 1, slot >= 1 ? slot - 1 : T::STAGES - 1);                          \
+    __builtin_amdgcn_sched_barrier(0);                                                                      \
+    vmcnt_wait<OUT>();                                                                                      \
+    lds_barrier();                                                                                          \
+    __builtin_amdgcn_sched_barrier(0);                                                                      \
+    __builtin_amdgcn_s_setprio(1);                                                                          \
+    _Pragma("unroll") for (int i = 0; i < TX; ++i) _Pragma("unroll") for (int j = 0; j < TW; ++j)           \
+        acc[i][j] = mfma32<S, 2 * H>(a[j], b[i][0], b[i][1], acc[i][j], sw[j][H], sx[i][S]);                \
+    __builtin_amdgcn_s_setprio(0);                                                                          \
+    __builtin_amdgcn_sched_barrier(0);                                                                      \
+    lds_barrier();                                                                                          \
+    __builtin_amdgcn_sched_barrier(0);                                                                      \
+    slot = slot + 1 < T::STAGES ? slot + 1 : 0;                                                             \
   }
-  for (int kt = 0;; kt += 4) {
+#define QE_STEP(S) QE_HALF(S, 0) QE_HALF(S, 1)
+  int kt = 0;
+  for (; kt + 4 <= KT; kt += 4) {
     take(kt / 4);
     QE_STEP(0) QE_STEP(1) QE_STEP(2) QE_STEP(3)
   }
+  if (kt < KT) {  // the last one to three steps: a loop with exits between would wait for all loads at each of them
+    take(kt / 4);
+    QE_STEP(0)
+    if (kt + 1 < KT) { QE_STEP(1) }
+    if (kt + 2 < KT) { QE_STEP(2) }
+  }
 #undef QE_STEP
+#undef QE_HALF
+  if (!second) lds_barrier();
 
   // out: a wave's 32 rows at a time through LDS, so that a row's neighbouring values leave in 16-byte stores
 #pragma unroll
