@@ -28,7 +28,7 @@ ARCH = "gfx950"
 HIP_SOURCES = ["attn_prep.hip", "attn_decode.hip", "attn_combine.hip", "attn_prefill.hip",
                "attn_prefill_wide.hip", "attn_paged.hip", "attn_prep_paged.hip", "kv_pages.hip",
                "gemv.hip", "gemv_lds.hip", "step.hip", "gdn.hip", "gdn_split.hip",
-               "mx_weight.hip", "mx_rows.hip", "mx_gemm.hip", "mx_gemm_tile.hip"]
+               "mx_weight.hip", "mx_rows.hip", "mx_gemm.hip", "mx_gemm_block.hip", "mx_gemm_tile.hip"]
 # Per-source code-generation flags. The prefill tile loop keeps 128 fp32 accumulators live; the
 # compiler's default MFMA register form parks them in AGPRs and copies all of them into VGPRs
 # on every iteration. The VGPR form keeps them in place. The max-ILP machine scheduler keeps
@@ -41,6 +41,8 @@ MAX_ILP = ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]
 SOURCE_FLAGS = {"attn_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", *MAX_ILP],
                 "attn_prefill_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", *MAX_ILP],
                 "attn_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+                "mx_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+                "mx_gemm_block.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                 "mx_gemm_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                 "attn_combine.hip": MAX_ILP, "gdn_split.hip": MAX_ILP, "gemv_lds.hip": MAX_ILP}
 BINDINGS = ["bindings", "bindings_paged", "bindings_mx"]  # .cpp

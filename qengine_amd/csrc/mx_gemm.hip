@@ -1,75 +1,200 @@
 // The product of 8-bit rows and a 4-bit weight (microscaled formats) on gfx950's scaled matrix instructions: codes
-// and scales go into them as they lie in memory, no value is converted.
+// and scales go into them as they lie in memory, no value is converted. The kernel for up to 16 rows (and small
+// products of more), and the choice between it and those of mx_gemm_block.hip and mx_gemm_tile.hip.
+#include <stdint.h>
+
+#include <algorithm>
+#include <cmath>
+
 #include "mx_common.hpp"
 #include "mx_gemm.hpp"
 
 namespace qe {
 namespace mx {
 
-typedef int i32x8_t __attribute__((ext_vector_type(8)));
+// ------------------------------------------------------------------------------ up to 16 rows
+// Streams the weight. A workgroup takes MT tiles of 16 weight rows; its waves, as many as K has groups of 512 values, or
+// a whole fraction of that (at most 16), share K by groups and their sums are added in order. A column of the product is one
+// row of x, which no other column touches, and the split goes by K alone: a row's bits do not depend on the others.
+constexpr int ROW_WAVES = 16;
 
-// D (16 x 16) += A (16 weight rows x 128) * B (128 x 16 rows), A E2M1 and B E4M3 codes. Lane r + 16 g: A's row r,
-// block g (16 bytes); B's row r at 16 g .. 16 g + 15 and 64 + 16 g .. 64 + 16 g + 15; the scales of A's and of B's row r,
-// block g (byte T of `sa`, byte 0 of `sb`). It gets D's rows 4 g .. 4 g + 3 of column r.
-template <int T>
-__device__ __forceinline__ f32x4_t mfma_mx(u32x4_t a, u32x4_t b0, u32x4_t b1, f32x4_t d, uint32_t sa, uint32_t sb) {
-  const i32x8_t A = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
-  const i32x8_t B = {(int)b0[0], (int)b0[1], (int)b0[2], (int)b0[3], (int)b1[0], (int)b1[1], (int)b1[2], (int)b1[3]};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, d, 4, 0, T, (int)sa, 0, (int)sb);
-}
-
-constexpr int WAVES = 8;
-
-template <int NT>
-__global__ void __launch_bounds__(WAVES * WAVE)
-gemm_mx4_kernel(const uint8_t* __restrict__ wq, const uint8_t* __restrict__ xq, long ldx,
-                const uint8_t* __restrict__ xs, long lds, __bf16* __restrict__ out, long ldo, int n, int N, int K) {
-  __shared__ f32x4_t part[WAVES][NT][WAVE];
+template <int MT, bool ONE>
+__global__ void __launch_bounds__(ROW_WAVES * WAVE, 4)
+gemm_mx4_rows_kernel(const uint8_t* wq, const uint8_t* xq, long ldx, const uint8_t* xs, long lds, __bf16* out,
+                     long ldo, int n, int N, int K, int per) {
+  __shared__ f32x4_t part[ROW_WAVES][MT][WAVE];
   const Layout L(N, K);
-  const int lane = threadIdx.x & (WAVE - 1), r = lane & 15, g = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  const int rt = blockIdx.x, col = blockIdx.y * 16 * NT;
-  f32x4_t acc[NT];
-  const uint8_t *xr[NT], *sr[NT];
+  const int lane = threadIdx.x & (WAVE - 1), r = lane & 15, g = lane >> 4, Kb = K / BLOCK;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE;
+  const int rt = blockIdx.x * MT, col = blockIdx.y * 16;
+  const int beg = w * per, end = min(beg + per, L.KS);
+  const bool live = col + r < n;
+  const int rows = min(16, n - col);
+  const uint32_t tiles = (uint32_t)min(MT, L.RT - rt);
+  // what lies past the row's end, rows past n and weight rows past N read as zeros: they lie outside the buffers
+  const __amdgpu_buffer_rsrc_t wr = make_rsrc_uniform(wq + (size_t)rt * L.KT * 1024, tiles * L.KT * 1024u);
+  const __amdgpu_buffer_rsrc_t ar = make_rsrc_uniform(wq + L.scales() + (size_t)rt * L.KS * 256, tiles * L.KS * 256u);
+  const __amdgpu_buffer_rsrc_t xr =
+      make_rsrc_uniform(xq + (size_t)col * ldx, (uint32_t)((size_t)(rows - 1) * ldx + K));
+  const uint32_t off = live ? 0u : 0x80000000u;
+  const uint32_t xo = (uint32_t)(r * ldx) + 16 * g;
+  const uint8_t* sr = xs + (size_t)(col + min(r, rows - 1)) * lds;
+  f32x4_t acc[MT];
+  u32x4_t a[MT][4], b[4][2], sb;
+  uint32_t sa[MT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const size_t row = min(col + 16 * i + r, n - 1);
-    xr[i] = xq + row * ldx;
-    sr[i] = xs + row * lds;
-  }
-  for (int J = w; J < L.KS; J += WAVES) {
-    const uint32_t sa = reinterpret_cast<const uint32_t*>(wq + L.scales() + ((size_t)rt * L.KS + J) * 256)[lane];
-#define QE_STEP(T)                                                                                               \
-  if (J * 4 + T < L.KT) {                                                                                        \
-    const int kt = J * 4 + T, k = kt * 128 + 16 * g;                                                             \
-    const u32x4_t a = reinterpret_cast<const u32x4_t*>(wq + ((size_t)rt * L.KT + kt) * 1024)[lane];              \
-    _Pragma("unroll") for (int i = 0; i < NT; ++i) {                                                             \
-      u32x4_t b0 = {0u, 0u, 0u, 0u}, b1 = {0u, 0u, 0u, 0u};                                                      \
-      uint32_t sb = 0;                                                                                           \
-      if (k < K) b0 = *reinterpret_cast<const u32x4_t*>(xr[i] + k);                                              \
-      if (k + 64 < K) b1 = *reinterpret_cast<const u32x4_t*>(xr[i] + k + 64);                                    \
-      if (kt * 4 + g < K / BLOCK) sb = sr[i][kt * 4 + g];                                                        \
-      acc[i] = mfma_mx<T>(a, b0, b1, acc[i], sa, sb);                                                            \
-    }                                                                                                            \
-  }
-    QE_STEP(0) QE_STEP(1) QE_STEP(2) QE_STEP(3)
-#undef QE_STEP
+  for (int m = 0; m < MT; ++m) acc[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  auto load = [&](int J) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        a[m][t] = buffer_load16_stream(
+            wr, (uint32_t)((m * L.KT + J * 4 + t) * 1024 + lane * 16) | (J * 4 + t < L.KT ? 0u : 0x80000000u));
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+      sa[m] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(ar, (m * L.KS + J) * 256 + lane * 4, 0, 0);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = J * 512 + t * 128 + h * 64;
+        b[t][h] = buffer_load16(xr, (xo + k) | off | (k + 16 * g < K ? 0u : 0x80000000u));
+      }
+    // the group's 16 scales of a row; the last group's come from the row's end, shifted down below
+    if (!ONE || Kb >= 16) {
+      __builtin_memcpy(&sb, sr + min(J * 16, Kb - 16), 16);
+    } else {
+      sb = u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t v = sr[min(e, Kb - 1)];
+        sb[e / 4] |= (e < Kb ? v : 0u) << (8 * (e & 3));
+      }
+    }
+  };
+  auto multiply = [&](int J) {
+    const int cut = J * 16 - (Kb - 16);  // bytes
+    if ((!ONE || Kb >= 16) && cut > 0) {
+      uint64_t lo = (uint64_t)sb[1] << 32 | sb[0], hi = (uint64_t)sb[3] << 32 | sb[2];
+      if (cut >= 8) lo = hi, hi = 0;
+      const int bits = (cut & 7) * 8;
+      lo = lo >> bits | (bits ? hi << (64 - bits) : 0);
+      hi >>= bits;
+      sb = u32x4_t{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+    }
+#define QE_TILE(T)                                                                  \
+  _Pragma("unroll") for (int m = 0; m < MT; ++m) acc[m] =                           \
+      mfma16<T>(a[m][T], b[T][0], b[T][1], acc[m], sa[m], sb[T] >> (8 * g));
+    QE_TILE(0) QE_TILE(1) QE_TILE(2) QE_TILE(3)
+#undef QE_TILE
+  };
+  // the other waves' loads are in flight while one multiplies
+  if constexpr (ONE) {
+    load(beg);
+    multiply(beg);
+  } else {
+    for (int J = beg; J < end; ++J) {
+      load(J);
+      multiply(J);
+    }
   }
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    asm volatile("" : "+v"(acc[i]));  // the products stay out of the stores' branches, where lanes are off
-    part[w][i][lane] = acc[i];
+  for (int m = 0; m < MT; ++m) {
+    asm volatile("" : "+v"(acc[m]));  // the products stay out of branches in which lanes are off
+    part[w][m][lane] = acc[m];
   }
   __syncthreads();
-  for (int i = w; i < NT; i += WAVES) {
-    f32x4_t t = part[0][i][lane];
-    for (int p = 1; p < WAVES; ++p) t += part[p][i][lane];
-    const int row = col + 16 * i + r, j = rt * 16 + 4 * g;
-    if (row < n)
-      for (int e = 0; e < 4; ++e)
-        if (j + e < N) out[(size_t)row * ldo + j + e] = f32_to_bf16(t[e]);
+  for (int m = w; m < MT; m += waves) {
+    f32x4_t t = part[0][m][lane];
+    for (int p = 1; p < waves; ++p) t += part[p][m][lane];
+    const int j = (rt + m) * 16 + 4 * g;
+    if (live && j < N) store4(out + (size_t)(col + r) * ldo + j, N - j, t);
   }
+}
+
+static hipError_t gemm_rows(const Product& c, hipStream_t stream) {
+  const Layout L(c.N, c.K);
+  const int per = (L.KS + ROW_WAVES - 1) / ROW_WAVES, waves = (L.KS + per - 1) / per, xt = (c.n + 15) / 16;
+  const long units = (long)L.RT * xt, cus = compute_units();
+  const int mt = c.n > 8 && units >= 3 * cus ? 4 : 4 * units >= 5 * cus ? 2 : 1;
+  const dim3 grid((L.RT + mt - 1) / mt, xt), block(waves * WAVE);
+#define QE_RUN(...) \
+  __VA_ARGS__<<<grid, block, 0, stream>>>(c.wq, c.xq, c.ldx, c.xs, c.lds, c.out, c.ldo, c.n, c.N, c.K, per)
+  if (per == 1) {
+    if (mt == 1) QE_RUN(gemm_mx4_rows_kernel<1, true>);
+    else if (mt == 2) QE_RUN(gemm_mx4_rows_kernel<2, true>);
+    else QE_RUN(gemm_mx4_rows_kernel<4, true>);
+  } else {
+    if (mt == 1) QE_RUN(gemm_mx4_rows_kernel<1, false>);
+    else if (mt == 2) QE_RUN(gemm_mx4_rows_kernel<2, false>);
+    else QE_RUN(gemm_mx4_rows_kernel<4, false>);
+  }
+#undef QE_RUN
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------- which kernel
+struct Choice {
+  enum { ROWS, BLOCK_KERNEL, TILE } kernel;
+  BlockKind block;
+  int splits;
+  TileKind tile;
+};
+
+static size_t split_bytes(int n, int N, int splits) {
+  return splits > 1 ? (size_t)splits * n * ((N + 15) / 16 * 16) * 4 : 0;
+}
+
+// Up to 16 rows always go to the streaming kernel, or a row's bits would depend on the others. More rows do where the
+// work is small and K short (us, it / the best of the others: 32 x 1000 x 1000 3.9 / 5.6, 102 x 171 x 2176 4.6 / 6.8;
+// past the rule 25 x 13906 x 128 4.8 / 5.4, 55 x 15157 x 352 8.2 / 6.9, 17 x 5120 x 6144 9.6 / 8.9).
+// Between the others decides what each would take, in us: what a call costs at once, steps of 128 of K of the
+// workgroups that take turns on a CU, and outputs (MB; a split writes and reads fp32 instead). The constants are least
+// squares over 130 calls from 17 x 18 x 64 to 2048 x 34816 x 5120, on which the choice is 6 % behind the best of the
+// five kernels and their splits (us, 256 x 256 / 256 x 160 / 128 x 256 / 64 x 128 / 32 x 64): 2048 x 34816 x 5120
+// 282 / 300 / 336 / 499 / 1215, 2048 x 5120 x 6144 62 / 50 / 67 / 80 / 183, 1024 x 5120 x 5120 49 / 36 / 31 / 37 / 82,
+// 300 x 5120 x 6144 53 / 38 / 32 / 16 / 28, 77 x 5001 x 6176 55 / 39 / 34 / 21 / 13. Splits: 128 x 5120 x 17408 on
+// 64 x 128, 33 us in one part, 24 in 2, 27 in 4; 19 x 20 x 9376 on 32 x 64, 11.4 us in one, 8.2 in 8.
+static Choice choose(int n, int N, int K, size_t ws_bytes) {
+  const Layout L(N, K);
+  const long units = (long)((n + 15) / 16) * L.RT;
+  if (n <= 16 || (L.KS <= ROW_WAVES && units * L.KS <= 2000)) return {Choice::ROWS, {}, 1, {}};
+  const double cus = compute_units(), mb = 2e-6 * n * N;
+  Choice best = {Choice::TILE, {}, 1, TileKind::X256_W256};
+  double least = 1e30;
+  struct TileCost {
+    int rows, cols;
+    double fixed, step, busy, out;
+  };
+  static const TileCost tile_cost[(int)TileKind::COUNT] = {
+      {256, 256, 10.6, 0.90, 0.16, 0.42}, {128, 256, 8.8, 0.48, 0.17, 0.40}, {256, 160, 8.7, 0.60, 0.18, 0.40}};
+  for (int i = 0; i < (int)TileKind::COUNT; ++i) {
+    const TileCost& c = tile_cost[i];
+    const double tiles = (double)((n + c.rows - 1) / c.rows) * ((N + c.cols - 1) / c.cols);
+    const double steps = std::ceil(tiles / cus) * std::max(L.KT, 2);
+    const double us = c.fixed + steps * (c.step + c.busy * std::min(tiles / cus, 1.)) + c.out * mb;
+    if (us < least) least = us, best = {Choice::TILE, {}, 1, (TileKind)i};
+  }
+  struct BlockCost {
+    int rows, cols;
+    double fixed, step, turn, sum, out;
+  };
+  static const BlockCost block_cost[(int)BlockKind::COUNT] = {{64, 128, 4.1, 0.23, 2.2, 1.8, 0.28},
+                                                              {32, 64, 3.8, 0.44, 2.4, 1.8, 0.24}};
+  for (int i = 0; i < (int)BlockKind::COUNT; ++i) {
+    const BlockCost& c = block_cost[i];
+    const double tiles = (double)((n + c.rows - 1) / c.rows) * ((N + c.cols - 1) / c.cols);
+    for (int splits = 1; splits <= 8; splits *= 2) {
+      const Parts k = block_parts((BlockKind)i, K, splits);
+      if (k.splits != splits || split_bytes(n, N, splits) > ws_bytes) continue;
+      const double turns = tiles * splits / cus;
+      const double us = c.fixed + std::max(turns, 1.) * k.part * c.step + turns * c.turn +
+                        (splits > 1 ? c.sum + c.out * mb * (2 * splits + 1) : c.out * mb);
+      if (us < least) least = us, best = {Choice::BLOCK_KERNEL, (BlockKind)i, splits, {}};
+    }
+  }
+  return best;
 }
 
 }  // namespace mx
@@ -78,22 +203,23 @@ gemm_mx4_kernel(const uint8_t* __restrict__ wq, const uint8_t* __restrict__ xq, 
 using namespace qe;
 using namespace qe::mx;
 
-extern "C" size_t qe_gemm_mx4_ws_size(int, int, int) { return 0; }
+extern "C" size_t qe_gemm_mx4_ws_size(int n, int N, int K) {
+  if (!dims_ok(n, 1) || !dims_ok(N, K) || K % BLOCK) return 0;
+  const Choice c = choose(n, N, K, SIZE_MAX);
+  return split_bytes(n, N, c.splits);
+}
 
 extern "C" hipError_t qe_gemm_mx4(const void* wq, const void* xq, long ldx, const void* xs, long lds, void* out,
-                                  long ldo, int n, int N, int K, void* ws, size_t, hipStream_t stream) {
+                                  long ldo, int n, int N, int K, void* ws, size_t ws_bytes, hipStream_t stream) {
   if (!wq || !xq || !xs || !out || !dims_ok(n, K) || !dims_ok(N, K) || K % BLOCK || !ld_ok(ldx, K) || ldx % 16 ||
-      !ld_ok(lds, K / BLOCK) || !ld_ok(ldo, N) || !aligned(wq, 16) || !aligned(xq, 16) || !aligned(out, 2) || !aligned(ws, 16))
+      !ld_ok(lds, K / BLOCK) || !ld_ok(ldo, N) || !aligned(wq, 16) || !aligned(xq, 16) || !aligned(out, 2) ||
+      !aligned(ws, 16))
     return hipErrorInvalidValue;
-  const int RT = Layout(N, K).RT;
-  const auto *W = static_cast<const uint8_t*>(wq), *X = static_cast<const uint8_t*>(xq),
-             *S = static_cast<const uint8_t*>(xs);
-  auto* O = static_cast<__bf16*>(out);
-  if (n <= 16)
-    gemm_mx4_kernel<1><<<dim3(RT), dim3(WAVES * WAVE), 0, stream>>>(W, X, ldx, S, lds, O, ldo, n, N, K);
-  else if (n > 128)
-    return gemm_tiles(W, X, ldx, S, lds, O, ldo, n, N, K, stream);
-  else
-    gemm_mx4_kernel<4><<<dim3(RT, (n + 63) / 64), dim3(WAVES * WAVE), 0, stream>>>(W, X, ldx, S, lds, O, ldo, n, N, K);
-  return hipGetLastError();
+  const Product p = {static_cast<const uint8_t*>(wq), static_cast<const uint8_t*>(xq),
+                     static_cast<const uint8_t*>(xs), static_cast<__bf16*>(out), static_cast<float*>(ws),
+                     ldx, lds, ldo, n, N, K};
+  const Choice c = choose(n, N, K, ws ? ws_bytes : 0);
+  if (c.kernel == Choice::ROWS) return gemm_rows(p, stream);
+  if (c.kernel == Choice::TILE) return gemm_tiles(c.tile, p, stream);
+  return gemm_blocks(c.block, c.splits, p, stream);
 }

@@ -1,13 +1,69 @@
-// The parts of the product of 8-bit rows and a 4-bit weight.
+// The parts of the product of 8-bit rows and a 4-bit weight: the scaled matrix instructions, and the kernel for many
+// rows.
 #pragma once
 #include "qe_device.hpp"
 
 namespace qe {
 namespace mx {
 
-// Many rows, in tiles (mx_gemm_tile.hip).
-hipError_t gemm_tiles(const uint8_t* wq, const uint8_t* xq, long ldx, const uint8_t* xs, long lds, __bf16* out,
-                      long ldo, int n, int N, int K, hipStream_t stream);
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ i32x8_t operand(u32x4_t lo, u32x4_t hi) {
+  return i32x8_t{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+
+// D (16 x 16) += A (16 weight rows x 128) * B (128 x 16 rows), A E2M1 and B E4M3 codes. Lane r + 16 g: A's row r, block
+// g (16 bytes); B's row r at 16 g .. 16 g + 15 and at 64 + 16 g .. 64 + 16 g + 15; in byte SA of sa and the lowest
+// byte of sb the scales of A's and of B's row r, block g. It gets D's rows 4 g .. 4 g + 3 of column r.
+// D is fp32, and the sums of eights; the products of eight neighbouring k are first cut to whole multiples of
+// 2^(e - 13), e the largest sum of two codes' exponents among the eight, which is the instruction's own doing.
+template <int SA>
+__device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b0, u32x4_t b1, f32x4_t d, uint32_t sa, uint32_t sb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(a, u32x4_t{0u, 0u, 0u, 0u}), operand(b0, b1), d, 4,
+                                                          0, SA, (int)sa, 0, (int)sb);
+}
+
+// The same for D (32 x 32), 64 values of K: lane r + 32 g has A's row r, block g; B's row r at 16 g .. and 32 + 16 g ..;
+// the scales of block g in byte SA of sa and byte SB of sb. It gets D's rows 8 e + 4 g .. 8 e + 4 g + 3, e = 0
+// .. 3, of column r.
+template <int SA, int SB>
+__device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b0, u32x4_t b1, f32x16_t d, uint32_t sa, uint32_t sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(a, u32x4_t{0u, 0u, 0u, 0u}), operand(b0, b1), d, 4,
+                                                         0, SA, (int)sa, SB, (int)sb);
+}
+
+// Up to four neighbouring outputs, at any address.
+__device__ __forceinline__ void store4(__bf16* o, int left, f32x4_t t) {
+  const u32x2_t v = {pack_bf16x2(t[0], t[1]), pack_bf16x2(t[2], t[3])};
+  if (left >= 4)
+    __builtin_memcpy(o, &v, 8);
+  else
+    for (int e = 0; e < 3; ++e)
+      if (e < left) o[e] = f32_to_bf16(t[e]);
+}
+
+// A call, its arguments checked.
+struct Product {
+  const uint8_t *wq, *xq, *xs;
+  __bf16* out;
+  float* ws;  // the splits' partial sums [split][n][16 RT], or null
+  long ldx, lds, ldo;
+  int n, N, K;
+};
+
+// The kernels for many rows (mx_gemm_tile.hip), by their tiles' rows of x and of the weight.
+enum class TileKind { X256_W256, X128_W256, X256_W160, COUNT };
+hipError_t gemm_tiles(TileKind kind, const Product& p, hipStream_t stream);
+
+// The kernels for some rows (mx_gemm_block.hip): tiles, and groups of waves that share K.
+enum class BlockKind { X64_W128, X32_W64_K4, COUNT };
+// K in parts of whole 512-value groups: 128-value tiles of a part, and the splits that hold any of K.
+struct Parts {
+  int part, splits;
+};
+Parts block_parts(BlockKind kind, int K, int splits);
+hipError_t gemm_blocks(BlockKind kind, int splits, const Product& p, hipStream_t stream);
 
 }  // namespace mx
 }  // namespace qe

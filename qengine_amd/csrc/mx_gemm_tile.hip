@@ -1,4 +1,6 @@
 // The product of 8-bit rows and a 4-bit weight for many rows: tiles of WX x TX x 32 rows by WW x TW x 32 weight rows.
+#include <limits.h>
+
 #include <algorithm>
 
 #include "mx_common.hpp"
@@ -7,41 +9,26 @@
 namespace qe {
 namespace mx {
 
-typedef int i32x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-
-template <int SA, int SB>
-__device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b0, u32x4_t b1, f32x16_t d, uint32_t sa, uint32_t sb) {
-  const i32x8_t A = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
-  const i32x8_t B = {(int)b0[0], (int)b0[1], (int)b0[2], (int)b0[3], (int)b1[0], (int)b1[1], (int)b1[2], (int)b1[3]};
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, d, 4, 0, SA, (int)sa, SB, (int)sb);
-}
-
 template <int WX, int WW, int TX, int TW>
 struct Tile {
   static constexpr int WAVES = WX * WW, ROWS = WX * TX * 32, COLS = WW * TW * 32;
   static constexpr int XB = ROWS * 128, STAGE = XB + COLS * 64;  // bytes of a stage: x, then the weight
   static constexpr int DX = (ROWS / 8 + WAVES - 1) / WAVES, DW = (COLS / 16 + WAVES - 1) / WAVES;  // a wave's loads
   static_assert(WAVES % 2 == 0, "a wave's loads of x are of one parity");
+  static constexpr int PER_CU = 3 * STAGE <= 81920 && TX * TW <= 2 ? 2 : 1;  // workgroups
   // on the way out a wave turns 32 rows of OUT values at a time around in its share of a stage
-  static constexpr int OUT = STAGE / WAVES >= 32 * 144 && TW % 2 == 0 ? 64 : 32, PITCH = OUT * 2 + 16;
+  static constexpr int OUT = STAGE / WAVES >= 32 * 144 && TW % 2 == 0 ? 64 : 32;
+  static constexpr int PITCH = OUT * 2 + (STAGE / WAVES >= 32 * (OUT * 2 + 16) ? 16 : 0);  // bytes
   static_assert(STAGE / WAVES >= 32 * PITCH, "its share holds them");
 };
 
-// The calls' sizes, and where a workgroup's tiles are.
-struct Call {
-  const uint8_t *wq, *xq, *xs;
-  __bf16* out;
-  long ldx, lds, ldo;
-  int n, N, K;
+struct Call : Product {
   int xtiles, tiles;
-  bool vec;  // 16-byte stores
 };
 
-template <int WX, int WW, int TX, int TW>
-__global__ void __launch_bounds__(WX * WW * WAVE, (WX * WW + 3) / 4)
+template <int WX, int WW, int TX, int TW, class T = Tile<WX, WW, TX, TW>>
+__global__ void __launch_bounds__(T::WAVES * WAVE, T::WAVES / 4 * T::PER_CU)
 gemm_mx4_tile_kernel(const Call c) {
-  using T = Tile<WX, WW, TX, TW>;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[3 * T::STAGE];
   const Layout L(c.N, c.K);
   const int lane = threadIdx.x & (WAVE - 1), r = lane & 31, g = lane >> 5;
@@ -59,7 +46,7 @@ gemm_mx4_tile_kernel(const Call c) {
   // x: 8 rows of 128 bytes a load; slot s of row i holds chunk s ^ (i / 2 % 8), so that 16 rows' reads of a chunk meet
   // no bank twice and the row's 128 bytes are one request. The weight: a 16-row tile's 1 KB a load. Rows and
   // chunks past the matrix are zeros: they lie outside the buffers.
-  const int chunk16 = ((lane & 7) ^ ((w & 1) * 4 + (lane >> 4))) * 16;
+  const int chunk16 = ((lane & 7) ^ ((min(w, T::ROWS / 8 - 1) & 1) * 4 + (lane >> 4))) * 16;
   uint32_t xo[T::DX], wo[T::DW], xl[T::DX], wl[T::DW];
 #pragma unroll
   for (int i = 0; i < T::DX; ++i) {
@@ -320,8 +307,8 @@ gemm_mx4_tile_kernel(const Call c) {
           const u32x4_t v = *reinterpret_cast<const u32x4_t*>(mine + pr * T::PITCH + pc * 16);
           __bf16* o = c.out + (size_t)min(row, c.n - 1) * c.ldo + col;
           if (row < c.n) {
-            if (c.vec && col + 8 <= c.N)
-              *reinterpret_cast<u32x4_t*>(o) = v;
+            if (col + 8 <= c.N)
+              __builtin_memcpy(o, &v, 16);  // at any address
             else
               for (int e = 0; e < 8; ++e)
                 if (col + e < c.N) reinterpret_cast<uint16_t*>(o)[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
@@ -343,19 +330,23 @@ gemm_mx4_tile_kernel(const Call c) {
 }
 
 template <int WX, int WW, int TX, int TW>
-static hipError_t run(const uint8_t* wq, const uint8_t* xq, long ldx, const uint8_t* xs, long lds, __bf16* out,
-                      long ldo, int n, int N, int K, hipStream_t stream) {
+static hipError_t run(const Product& p, hipStream_t stream) {
   using T = Tile<WX, WW, TX, TW>;
-  const int xt = (n + T::ROWS - 1) / T::ROWS, tiles = xt * ((N + T::COLS - 1) / T::COLS);
-  const Call c = {wq, xq, xs, out, ldx, lds, ldo, n, N, K, xt, tiles, ldo % 8 == 0 && aligned(out, 16)};
+  const long xt = (p.n + T::ROWS - 1) / T::ROWS, tiles = xt * ((p.N + T::COLS - 1) / T::COLS);
+  if (tiles > INT_MAX / 2) return hipErrorInvalidValue;  // more outputs than there is memory
+  const Call c = {p, (int)xt, (int)tiles};
   gemm_mx4_tile_kernel<WX, WW, TX, TW>
-      <<<dim3(std::min(tiles, compute_units())), dim3(T::WAVES * WAVE), 0, stream>>>(c);
+      <<<dim3(std::min((int)tiles, compute_units() * T::PER_CU)), dim3(T::WAVES * WAVE), 0, stream>>>(c);
   return hipGetLastError();
 }
 
-hipError_t gemm_tiles(const uint8_t* wq, const uint8_t* xq, long ldx, const uint8_t* xs, long lds, __bf16* out,
-                      long ldo, int n, int N, int K, hipStream_t stream) {
-  return run<4, 2, 2, 4>(wq, xq, ldx, xs, lds, out, ldo, n, N, K, stream);
+hipError_t gemm_tiles(TileKind kind, const Product& p, hipStream_t stream) {
+  switch (kind) {
+    case TileKind::X256_W256: return run<4, 2, 2, 4>(p, stream);
+    case TileKind::X128_W256: return run<4, 2, 1, 4>(p, stream);
+    case TileKind::X256_W160: return run<8, 1, 1, 5>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 }  // namespace mx
