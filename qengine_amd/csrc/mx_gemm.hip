@@ -148,14 +148,16 @@ static size_t split_bytes(int n, int N, int splits) {
 
 // Up to 16 rows always go to the streaming kernel, or a row's bits would depend on the others. More rows do where the
 // work is small and K short (us, it / the best of the others: 32 x 1000 x 1000 3.9 / 5.6, 102 x 171 x 2176 4.6 / 6.8;
-// past the rule 25 x 13906 x 128 4.8 / 5.4, 55 x 15157 x 352 8.2 / 6.9, 17 x 5120 x 6144 9.6 / 8.9).
-// Between the others decides what each would take, in us: what a call costs at once, steps of 128 of K of the
-// workgroups that take turns on a CU, and outputs (MB; a split writes and reads fp32 instead). The constants are least
-// squares over 130 calls from 17 x 18 x 64 to 2048 x 34816 x 5120, on which the choice is 6 % behind the best of the
-// five kernels and their splits (us, 256 x 256 / 256 x 160 / 128 x 256 / 64 x 128 / 32 x 64): 2048 x 34816 x 5120
-// 282 / 300 / 336 / 499 / 1215, 2048 x 5120 x 6144 62 / 50 / 67 / 80 / 183, 1024 x 5120 x 5120 49 / 36 / 31 / 37 / 82,
-// 300 x 5120 x 6144 53 / 38 / 32 / 16 / 28, 77 x 5001 x 6176 55 / 39 / 34 / 21 / 13. Splits: 128 x 5120 x 17408 on
-// 64 x 128, 33 us in one part, 24 in 2, 27 in 4; 19 x 20 x 9376 on 32 x 64, 11.4 us in one, 8.2 in 8.
+// past the rule 25 x 13906 x 128 4.8 / 5.4, 55 x 15157 x 352 8.2 / 6.9, 17 x 5120 x 6144 9.6 / 7.8).
+// Between the others decides what each would take, in us: what a call costs at once, the steps of 128 of K of the
+// workgroups that take turns on a CU (a little longer while every CU has one), a workgroup's start and end, and outputs
+// (MB; a split writes and reads fp32 as well). The constants are least squares over 150 calls from 17 x 18 x 64 to
+// 2048 x 34816 x 5120, on which the choice is 4 % behind the best kernel and split (us, tiles of 256 x 256 /
+// 256 x 160 / 128 x 256 / 64 x 256 / 64 x 128 / 32 x 64): 2048 x 34816 x 5120 282 / 300 / 336 / - / 499 / 1215,
+// 2048 x 5120 x 6144 62 / 50 / 67 / - / 80 / 183, 1024 x 5120 x 5120 49 / 34 / 29 / 38 / 35 / 82,
+// 64 x 34816 x 5120 46 / 38 / 37 / 31 / 39 / 48 (272 tiles of 64 x 128 on 256 CUs, 136 of 64 x 256),
+// 300 x 5120 x 6144 53 / 38 / 32 / 20 / 15 / 27, 77 x 5001 x 6176 55 / 39 / 34 / 21 / 16 / 11. Splits:
+// 128 x 5120 x 17408 on 64 x 128, 48 us in one part, 22 in 2, 25 in 4; 40 x 100 x 17408 on 32 x 64, 17 in one, 9.0 in 4.
 static Choice choose(int n, int N, int K, size_t ws_bytes) {
   const Layout L(N, K);
   const long units = (long)((n + 15) / 16) * L.RT;
@@ -163,37 +165,32 @@ static Choice choose(int n, int N, int K, size_t ws_bytes) {
   const double cus = compute_units(), mb = 2e-6 * n * N;
   Choice best = {Choice::TILE, {}, 1, TileKind::X256_W256};
   double least = 1e30;
-  struct TileCost {
+  struct Cost {
     int rows, cols;
-    double fixed, step, busy, out;
+    double call, step, full, group, split, out;
   };
-  static const TileCost tile_cost[(int)TileKind::COUNT] = {
-      {256, 256, 10.6, 0.90, 0.16, 0.42}, {128, 256, 8.8, 0.48, 0.17, 0.40}, {256, 160, 8.7, 0.60, 0.18, 0.40}};
+  static const Cost tile_cost[(int)TileKind::COUNT] = {{256, 256, 10.5, 0.90, 0.09, 0, 0, 0.37},
+                                                       {128, 256, 8.5, 0.47, 0.18, 0, 0, 0.29},
+                                                       {256, 160, 8.5, 0.59, 0.15, 0, 0, 0.34}};
+  static const Cost block_cost[(int)BlockKind::COUNT] = {{64, 128, 4.1, 0.21, 0.04, 1.0, 1.8, 0.31},
+                                                         {64, 256, 3.9, 0.34, 0.06, 1.4, 2.1, 0.34},
+                                                         {32, 64, 3.7, 0.39, 0.06, 1.8, 1.8, 0.28}};
+  auto cost = [&](const Cost& c, int steps, int splits) {
+    const double turns = (double)((n + c.rows - 1) / c.rows) * ((N + c.cols - 1) / c.cols) * splits / cus;
+    return c.call + std::ceil(turns) * steps * (c.step + c.full * std::min(turns, 1.)) + turns * c.group +
+           (splits > 1 ? c.split + c.out * mb * (2 * splits + 1) : c.out * mb);
+  };
   for (int i = 0; i < (int)TileKind::COUNT; ++i) {
-    const TileCost& c = tile_cost[i];
-    const double tiles = (double)((n + c.rows - 1) / c.rows) * ((N + c.cols - 1) / c.cols);
-    const double steps = std::ceil(tiles / cus) * std::max(L.KT, 2);
-    const double us = c.fixed + steps * (c.step + c.busy * std::min(tiles / cus, 1.)) + c.out * mb;
+    const double us = cost(tile_cost[i], std::max(L.KT, 2), 1);
     if (us < least) least = us, best = {Choice::TILE, {}, 1, (TileKind)i};
   }
-  struct BlockCost {
-    int rows, cols;
-    double fixed, step, turn, sum, out;
-  };
-  static const BlockCost block_cost[(int)BlockKind::COUNT] = {{64, 128, 4.1, 0.23, 2.2, 1.8, 0.28},
-                                                              {32, 64, 3.8, 0.44, 2.4, 1.8, 0.24}};
-  for (int i = 0; i < (int)BlockKind::COUNT; ++i) {
-    const BlockCost& c = block_cost[i];
-    const double tiles = (double)((n + c.rows - 1) / c.rows) * ((N + c.cols - 1) / c.cols);
+  for (int i = 0; i < (int)BlockKind::COUNT; ++i)
     for (int splits = 1; splits <= 8; splits *= 2) {
       const Parts k = block_parts((BlockKind)i, K, splits);
       if (k.splits != splits || split_bytes(n, N, splits) > ws_bytes) continue;
-      const double turns = tiles * splits / cus;
-      const double us = c.fixed + std::max(turns, 1.) * k.part * c.step + turns * c.turn +
-                        (splits > 1 ? c.sum + c.out * mb * (2 * splits + 1) : c.out * mb);
+      const double us = cost(block_cost[i], k.part, splits);
       if (us < least) least = us, best = {Choice::BLOCK_KERNEL, (BlockKind)i, splits, {}};
     }
-  }
   return best;
 }
 

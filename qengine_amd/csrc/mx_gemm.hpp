@@ -57,7 +57,7 @@ enum class TileKind { X256_W256, X128_W256, X256_W160, COUNT };
 hipError_t gemm_tiles(TileKind kind, const Product& p, hipStream_t stream);
 
 // The kernels for some rows (mx_gemm_block.hip): tiles, and groups of waves that share K.
-enum class BlockKind { X64_W128, X32_W64_K4, COUNT };
+enum class BlockKind { X64_W128, X64_W256, X32_W64_K4, COUNT };
 // K in parts of whole 512-value groups: 128-value tiles of a part, and the splits that hold any of K.
 struct Parts {
   int part, splits;

@@ -156,7 +156,11 @@ gemm_mx4_block_kernel(const BlockCall c) {
     }
   }
 #pragma unroll
-  for (int s = 0; s < T::ST; ++s) fetch(s, s);
+  for (int s = 0; s < T::ST; ++s) {
+    __builtin_amdgcn_sched_barrier(0);  // in this order: the waits below count them
+    fetch(s, s);
+  }
+  __builtin_amdgcn_sched_barrier(0);
   take(k0 / 4);
   u32x4_t a[2][2][TW], b[2][2][TX][2];
   auto read = [&](int stage, int to) {
@@ -177,29 +181,29 @@ gemm_mx4_block_kernel(const BlockCall c) {
   lds_barrier();
   read(0, 0);
   int stage = 0;
-  // A step, whose operands are in registers: behind its products the next step's are read (its stage has landed once only
-  // the ST - 2 after it are out, and scales that were loaded since), and the step ST ahead takes the place of
-  // this one, which every wave has read ahead of the barrier.
-#define QE_STEP(S)                                                                                           \
-  {                                                                                                          \
+  // A step, whose operands are in registers: the next step's are read behind the barrier (that stage has landed: only
+  // the ST - 2 steps after it are out, and scales loaded since), the loads of the step ST ahead take the place of
+  // this one, which every wave has read ahead of the barrier, and this step's products run meanwhile.
+#define QE_STEP(S)                                                                                            \
+  {                                                                                                           \
+    vmcnt_wait<(T::ST - 2) * T::LOADS + (S >= 1 && S <= T::ST - 2 ? SCALES : 0)>();                           \
+    lds_barrier();                                                                                            \
+    __builtin_amdgcn_sched_barrier(0);                                                                        \
+    const int next = stage + 1 < T::ST ? stage + 1 : 0;                                                       \
+    read(next, 1 - (S & 1));                                                                                  \
+    __builtin_amdgcn_sched_barrier(0);                                                                        \
+    if (S == 0) scales((k0 + s0) / 4 + 1);                                                                    \
+    __builtin_amdgcn_sched_barrier(0);                                                                        \
+    fetch(s0 + S + T::ST, stage);                                                                             \
+    __builtin_amdgcn_sched_barrier(0);                                                                        \
     _Pragma("unroll") for (int i = 0; i < TX; ++i) _Pragma("unroll") for (int j = 0; j < TW; ++j) acc[i][j] = \
-        mfma32<S, 0>(a[S & 1][0][j], b[S & 1][0][i][0], b[S & 1][0][i][1], acc[i][j], sw[j][0], sx[i][S]);   \
+        mfma32<S, 0>(a[S & 1][0][j], b[S & 1][0][i][0], b[S & 1][0][i][1], acc[i][j], sw[j][0], sx[i][S]);    \
     _Pragma("unroll") for (int i = 0; i < TX; ++i) _Pragma("unroll") for (int j = 0; j < TW; ++j) acc[i][j] = \
-        mfma32<S, 2>(a[S & 1][1][j], b[S & 1][1][i][0], b[S & 1][1][i][1], acc[i][j], sw[j][1], sx[i][S]);   \
-    _Pragma("unroll") for (int i = 0; i < TX; ++i) _Pragma("unroll") for (int j = 0; j < TW; ++j)            \
-        asm volatile("" : "+v"(acc[i][j]));                                                                  \
-    __builtin_amdgcn_sched_barrier(0);                                                                       \
-    vmcnt_wait<(T::ST - 2) * T::LOADS + (S >= 1 && S <= T::ST - 2 ? SCALES : 0)>();                          \
-    lds_barrier();                                                                                           \
-    __builtin_amdgcn_sched_barrier(0);                                                                       \
-    const int next = stage + 1 < T::ST ? stage + 1 : 0;                                                      \
-    read(next, 1 - (S & 1));                                                                                 \
-    __builtin_amdgcn_sched_barrier(0);                                                                       \
-    if (S == 0) scales((k0 + s0) / 4 + 1);                                                                   \
-    __builtin_amdgcn_sched_barrier(0);                                                                       \
-    fetch(s0 + S + T::ST, stage);                                                                            \
-    __builtin_amdgcn_sched_barrier(0);                                                                       \
-    stage = next;                                                                                            \
+        mfma32<S, 2>(a[S & 1][1][j], b[S & 1][1][i][0], b[S & 1][1][i][1], acc[i][j], sw[j][1], sx[i][S]);    \
+    _Pragma("unroll") for (int i = 0; i < TX; ++i) _Pragma("unroll") for (int j = 0; j < TW; ++j)             \
+        asm volatile("" : "+v"(acc[i][j]));                                                                   \
+    __builtin_amdgcn_sched_barrier(0);                                                                        \
+    stage = next;                                                                                             \
   }
   for (int s0 = 0; s0 < c.part; s0 += 4) {
     QE_STEP(0) QE_STEP(1) QE_STEP(2) QE_STEP(3)
@@ -283,12 +287,13 @@ static hipError_t run(const Product& p, int splits, hipStream_t stream) {
 }
 
 Parts block_parts(BlockKind kind, int K, int splits) {
-  return parts(kind == BlockKind::X64_W128 ? 1 : 4, K, splits);
+  return parts(kind == BlockKind::X32_W64_K4 ? 4 : 1, K, splits);
 }
 
 hipError_t gemm_blocks(BlockKind kind, int splits, const Product& p, hipStream_t stream) {
   switch (kind) {
     case BlockKind::X64_W128: return run<2, 4, 1, 1, 1, 4>(p, splits, stream);
+    case BlockKind::X64_W256: return run<2, 4, 1, 1, 2, 4>(p, splits, stream);
     case BlockKind::X32_W64_K4: return run<1, 2, 4, 1, 1, 3>(p, splits, stream);
     default: return hipErrorInvalidValue;
   }
