@@ -20,9 +20,9 @@ constexpr int ROW_WAVES = 16;
 
 template <int MT, bool ONE>
 __global__ void __launch_bounds__(ROW_WAVES * WAVE, 4)
-gemm_mx4_rows_kernel(const uint8_t* wq, const uint8_t* xq, long ldx, const uint8_t* xs, long lds, __bf16* out,
-                     long ldo, int n, int N, int K, int per) {
+gemm_mx4_rows_kernel(const Product c, int per) {
   __shared__ f32x4_t part[ROW_WAVES][MT][WAVE];
+  const int n = c.n, N = c.N, K = c.K;
   const Layout L(N, K);
   const int lane = threadIdx.x & (WAVE - 1), r = lane & 15, g = lane >> 4, Kb = K / BLOCK;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE;
@@ -32,13 +32,13 @@ gemm_mx4_rows_kernel(const uint8_t* wq, const uint8_t* xq, long ldx, const uint8
   const int rows = min(16, n - col);
   const uint32_t tiles = (uint32_t)min(MT, L.RT - rt);
   // what lies past the row's end, rows past n and weight rows past N read as zeros: they lie outside the buffers
-  const __amdgpu_buffer_rsrc_t wr = make_rsrc_uniform(wq + (size_t)rt * L.KT * 1024, tiles * L.KT * 1024u);
-  const __amdgpu_buffer_rsrc_t ar = make_rsrc_uniform(wq + L.scales() + (size_t)rt * L.KS * 256, tiles * L.KS * 256u);
+  const __amdgpu_buffer_rsrc_t wr = make_rsrc_uniform(c.wq + (size_t)rt * L.KT * 1024, tiles * L.KT * 1024u);
+  const __amdgpu_buffer_rsrc_t ar = make_rsrc_uniform(c.wscale + (size_t)rt * L.KS * 256, tiles * L.KS * 256u);
   const __amdgpu_buffer_rsrc_t xr =
-      make_rsrc_uniform(xq + (size_t)col * ldx, (uint32_t)((size_t)(rows - 1) * ldx + K));
+      make_rsrc_uniform(c.xq + (size_t)col * c.ldx, (uint32_t)((size_t)(rows - 1) * c.ldx + K));
   const uint32_t off = live ? 0u : 0x80000000u;
-  const uint32_t xo = (uint32_t)(r * ldx) + 16 * g;
-  const uint8_t* sr = xs + (size_t)(col + min(r, rows - 1)) * lds;
+  const uint32_t xo = (uint32_t)(r * c.ldx) + 16 * g;
+  const uint8_t* sr = c.xs + (size_t)(col + min(r, rows - 1)) * c.lds;
   f32x4_t acc[MT];
   u32x4_t a[MT][4], b[4][2], sb;
   uint32_t sa[MT];
@@ -109,7 +109,7 @@ gemm_mx4_rows_kernel(const uint8_t* wq, const uint8_t* xq, long ldx, const uint8
     f32x4_t t = part[0][m][lane];
     for (int p = 1; p < waves; ++p) t += part[p][m][lane];
     const int j = (rt + m) * 16 + 4 * g;
-    if (live && j < N) store4(out + (size_t)(col + r) * ldo + j, N - j, t);
+    if (live && j < N) store4(c.out + (size_t)(col + r) * c.ldo + j, N - j, t);
   }
 }
 
@@ -119,8 +119,7 @@ static hipError_t gemm_rows(const Product& c, hipStream_t stream) {
   const long units = (long)L.RT * xt, cus = compute_units();
   const int mt = c.n > 8 && units >= 3 * cus ? 4 : 4 * units >= 5 * cus ? 2 : 1;
   const dim3 grid((L.RT + mt - 1) / mt, xt), block(waves * WAVE);
-#define QE_RUN(...) \
-  __VA_ARGS__<<<grid, block, 0, stream>>>(c.wq, c.xq, c.ldx, c.xs, c.lds, c.out, c.ldo, c.n, c.N, c.K, per)
+#define QE_RUN(...) __VA_ARGS__<<<grid, block, 0, stream>>>(c, per)
   if (per == 1) {
     if (mt == 1) QE_RUN(gemm_mx4_rows_kernel<1, true>);
     else if (mt == 2) QE_RUN(gemm_mx4_rows_kernel<2, true>);
@@ -134,18 +133,7 @@ static hipError_t gemm_rows(const Product& c, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// ---------------------------------------------------------------------------- which kernel
-struct Choice {
-  enum { ROWS, BLOCK_KERNEL, TILE } kernel;
-  BlockKind block;
-  int splits;
-  TileKind tile;
-};
-
-static size_t split_bytes(int n, int N, int splits) {
-  return splits > 1 ? (size_t)splits * n * ((N + 15) / 16 * 16) * 4 : 0;
-}
-
+// ------------------------------------------------------------------------------ which kernel
 // Up to 16 rows always go to the streaming kernel, or a row's bits would depend on the others. More rows do where the
 // work is small and K short (us, it / the best of the others: 32 x 1000 x 1000 3.9 / 5.6, 102 x 171 x 2176 4.6 / 6.8;
 // past the rule 25 x 13906 x 128 4.8 / 5.4, 55 x 15157 x 352 8.2 / 6.9, 17 x 5120 x 6144 9.6 / 7.8).
@@ -158,39 +146,78 @@ static size_t split_bytes(int n, int N, int splits) {
 // 64 x 34816 x 5120 46 / 38 / 37 / 31 / 39 / 48 (272 tiles of 64 x 128 on 256 CUs, 136 of 64 x 256),
 // 300 x 5120 x 6144 53 / 38 / 32 / 20 / 15 / 27, 77 x 5001 x 6176 55 / 39 / 34 / 21 / 16 / 11. Splits:
 // 128 x 5120 x 17408 on 64 x 128, 48 us in one part, 22 in 2, 25 in 4; 40 x 100 x 17408 on 32 x 64, 17 in one, 9.0 in 4.
+struct Cost {
+  int rows, cols;  // of a tile
+  double call, step, full, group, split, out;
+};
+constexpr int TILES = (int)TileKind::COUNT, KINDS = TILES + (int)BlockKind::COUNT;
+static const Cost costs[KINDS] = {{256, 256, 10.5, 0.90, 0.09, 0.0, 0.0, 0.37},  // in TileKind's order
+                                  {128, 256, 8.5, 0.47, 0.18, 0.0, 0.0, 0.29},
+                                  {256, 160, 8.5, 0.59, 0.15, 0.0, 0.0, 0.34},
+                                  {64, 128, 4.1, 0.21, 0.04, 1.0, 1.8, 0.31},  // in BlockKind's
+                                  {64, 256, 3.9, 0.34, 0.06, 1.4, 2.1, 0.34},
+                                  {32, 64, 3.7, 0.39, 0.06, 1.8, 1.8, 0.28}};
+
+constexpr int ROWS = -1;
+struct Choice {
+  int kind;  // ROWS, or an index into costs
+  int splits;
+  double us;
+};
+
+static long tiles(const Cost& c, int n, int N) {
+  return (long)((n + c.rows - 1) / c.rows) * ((N + c.cols - 1) / c.cols);
+}
+
+static double estimate(int kind, int splits, int n, int N, int K) {
+  const Cost& c = costs[kind];
+  const double cus = compute_units(), turns = (double)tiles(c, n, N) * splits / cus, mb = 2e-6 * n * N;
+  const int steps = kind < TILES ? std::max((K + 127) / 128, 2) : block_parts((BlockKind)(kind - TILES), K, splits).part;
+  return c.call + std::ceil(turns) * steps * (c.step + c.full * std::min(turns, 1.)) + turns * c.group +
+         (splits > 1 ? c.split + c.out * mb * (2 * splits + 1) : c.out * mb);
+}
+
+static size_t split_bytes(int n, int N, int splits) {
+  return splits > 1 ? (size_t)splits * n * ((N + 15) / 16 * 16) * 4 : 0;
+}
+
 static Choice choose(int n, int N, int K, size_t ws_bytes) {
   const Layout L(N, K);
-  const long units = (long)((n + 15) / 16) * L.RT;
-  if (n <= 16 || (L.KS <= ROW_WAVES && units * L.KS <= 2000)) return {Choice::ROWS, {}, 1, {}};
-  const double cus = compute_units(), mb = 2e-6 * n * N;
-  Choice best = {Choice::TILE, {}, 1, TileKind::X256_W256};
-  double least = 1e30;
-  struct Cost {
-    int rows, cols;
-    double call, step, full, group, split, out;
-  };
-  static const Cost tile_cost[(int)TileKind::COUNT] = {{256, 256, 10.5, 0.90, 0.09, 0, 0, 0.37},
-                                                       {128, 256, 8.5, 0.47, 0.18, 0, 0, 0.29},
-                                                       {256, 160, 8.5, 0.59, 0.15, 0, 0, 0.34}};
-  static const Cost block_cost[(int)BlockKind::COUNT] = {{64, 128, 4.1, 0.21, 0.04, 1.0, 1.8, 0.31},
-                                                         {64, 256, 3.9, 0.34, 0.06, 1.4, 2.1, 0.34},
-                                                         {32, 64, 3.7, 0.39, 0.06, 1.8, 1.8, 0.28}};
-  auto cost = [&](const Cost& c, int steps, int splits) {
-    const double turns = (double)((n + c.rows - 1) / c.rows) * ((N + c.cols - 1) / c.cols) * splits / cus;
-    return c.call + std::ceil(turns) * steps * (c.step + c.full * std::min(turns, 1.)) + turns * c.group +
-           (splits > 1 ? c.split + c.out * mb * (2 * splits + 1) : c.out * mb);
-  };
-  for (int i = 0; i < (int)TileKind::COUNT; ++i) {
-    const double us = cost(tile_cost[i], std::max(L.KT, 2), 1);
-    if (us < least) least = us, best = {Choice::TILE, {}, 1, (TileKind)i};
-  }
-  for (int i = 0; i < (int)BlockKind::COUNT; ++i)
-    for (int splits = 1; splits <= 8; splits *= 2) {
-      const Parts k = block_parts((BlockKind)i, K, splits);
-      if (k.splits != splits || split_bytes(n, N, splits) > ws_bytes) continue;
-      const double us = cost(block_cost[i], k.part, splits);
-      if (us < least) least = us, best = {Choice::BLOCK_KERNEL, (BlockKind)i, splits, {}};
+  if (n <= 16 || (L.KS <= ROW_WAVES && (long)((n + 15) / 16) * L.RT * L.KS <= 2000)) return {ROWS, 1, 0.};
+  Choice best = {ROWS, 1, 1e30};
+  for (int kind = 0; kind < KINDS; ++kind)
+    for (int splits = 1; splits <= (kind < TILES ? 1 : 8); splits *= 2) {
+      if (splits > 1 && (block_parts((BlockKind)(kind - TILES), K, splits).splits != splits ||
+                         split_bytes(n, N, splits) > ws_bytes))
+        continue;
+      const double us = estimate(kind, splits, n, N, K);
+      if (us < best.us) best = {kind, splits, us};
     }
+  return best;
+}
+
+// A call, or two: the weight rows whose tiles give every CU the same number, and the others by what suits them (two
+// launches: by 3 % at least). 2048 x 34816 x 5120 is 1088 tiles of 256 x 256, 4.25 a CU: 282 us, with the last 2048
+// weight rows in 256 blocks of 64 x 256 271 us; 1024 x 34816 x 5120 163 and 142 us.
+struct Plan {
+  Choice first, rest;
+  int cut;  // weight rows of the first; N if that is all
+};
+
+static Plan plan(int n, int N, int K, size_t ws_bytes) {
+  Plan best = {choose(n, N, K, ws_bytes), {}, N};
+  if (best.first.kind == ROWS) return best;
+  double least = 0.97 * best.first.us;
+  const long cus = compute_units();
+  for (int kind = 0; kind < KINDS; ++kind) {
+    const long all = tiles(costs[kind], n, N), xtiles = (n + costs[kind].rows - 1) / costs[kind].rows;
+    const long cut = all / cus * cus / xtiles * costs[kind].cols;  // a multiple of 32
+    if (cut <= 0 || cut >= N) continue;
+    const double us = estimate(kind, 1, n, (int)cut, K);
+    if (us >= least) continue;
+    const Choice rest = choose(n, N - (int)cut, K, ws_bytes);
+    if (us + rest.us < least) least = us + rest.us, best = {{kind, 1, us}, rest, (int)cut};
+  }
   return best;
 }
 
@@ -202,8 +229,14 @@ using namespace qe::mx;
 
 extern "C" size_t qe_gemm_mx4_ws_size(int n, int N, int K) {
   if (!dims_ok(n, 1) || !dims_ok(N, K) || K % BLOCK) return 0;
-  const Choice c = choose(n, N, K, SIZE_MAX);
-  return split_bytes(n, N, c.splits);
+  const Plan p = plan(n, N, K, SIZE_MAX);
+  return p.cut < N ? split_bytes(n, N - p.cut, p.rest.splits) : split_bytes(n, N, p.first.splits);
+}
+
+static hipError_t run(const Choice& c, const Product& p, hipStream_t stream) {
+  if (c.kind == ROWS) return gemm_rows(p, stream);
+  if (c.kind < TILES) return gemm_tiles((TileKind)c.kind, p, stream);
+  return gemm_blocks((BlockKind)(c.kind - TILES), c.splits, p, stream);
 }
 
 extern "C" hipError_t qe_gemm_mx4(const void* wq, const void* xq, long ldx, const void* xs, long lds, void* out,
@@ -212,11 +245,21 @@ extern "C" hipError_t qe_gemm_mx4(const void* wq, const void* xq, long ldx, cons
       !ld_ok(lds, K / BLOCK) || !ld_ok(ldo, N) || !aligned(wq, 16) || !aligned(xq, 16) || !aligned(out, 2) ||
       !aligned(ws, 16))
     return hipErrorInvalidValue;
-  const Product p = {static_cast<const uint8_t*>(wq), static_cast<const uint8_t*>(xq),
-                     static_cast<const uint8_t*>(xs), static_cast<__bf16*>(out), static_cast<float*>(ws),
-                     ldx, lds, ldo, n, N, K};
-  const Choice c = choose(n, N, K, ws ? ws_bytes : 0);
-  if (c.kernel == Choice::ROWS) return gemm_rows(p, stream);
-  if (c.kernel == Choice::TILE) return gemm_tiles(c.tile, p, stream);
-  return gemm_blocks(c.block, c.splits, p, stream);
+  const Layout L(N, K);
+  Product p = {static_cast<const uint8_t*>(wq),
+               static_cast<const uint8_t*>(wq) + L.scales(),
+               static_cast<const uint8_t*>(xq),
+               static_cast<const uint8_t*>(xs),
+               static_cast<__bf16*>(out),
+               static_cast<float*>(ws),
+               ldx, lds, ldo, n, N, K};
+  const Plan how = plan(n, N, K, ws ? ws_bytes : 0);
+  p.N = how.cut;
+  const hipError_t e = run(how.first, p, stream);
+  if (e != hipSuccess || how.cut == N) return e;
+  p.wq += (size_t)(how.cut / 16) * L.KT * 1024;
+  p.wscale += (size_t)(how.cut / 16) * L.KS * 256;
+  p.out += how.cut;
+  p.N = N - how.cut;
+  return run(how.rest, p, stream);
 }

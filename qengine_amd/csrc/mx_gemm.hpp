@@ -45,7 +45,7 @@ __device__ __forceinline__ void store4(__bf16* o, int left, f32x4_t t) {
 
 // A call, its arguments checked.
 struct Product {
-  const uint8_t *wq, *xq, *xs;
+  const uint8_t *wq, *wscale, *xq, *xs;  // the weight's codes and its scales (of N rows on, where a call is cut)
   __bf16* out;
   float* ws;  // the splits' partial sums [split][n][16 RT], or null
   long ldx, lds, ldo;

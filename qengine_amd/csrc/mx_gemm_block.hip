@@ -87,7 +87,7 @@ gemm_mx4_block_kernel(const BlockCall c) {
   constexpr int SCALES = 2 * TW + TX;
   const bool small = Kb < 16;
   const int last16 = small ? 0 : Kb - 16;
-  const __amdgpu_buffer_rsrc_t sr = make_rsrc_uniform(c.wq + L.scales() + (size_t)rt0 * L.KS * 256,
+  const __amdgpu_buffer_rsrc_t sr = make_rsrc_uniform(c.wscale + (size_t)rt0 * L.KS * 256,
                                                       (uint32_t)min(T::COLS / 16, L.RT - rt0) * L.KS * 256u);
   const uint32_t so = (uint32_t)(ww * TW * 2 + (r >> 4)) * L.KS * 256u + ((r & 15) + 16 * g) * 4;
   const uint8_t *xp[TX], *xp16[TX];
