@@ -183,7 +183,7 @@ static size_t split_bytes(int n, int N, int splits) {
 
 static Choice choose(int n, int N, int K, size_t ws_bytes) {
   const Layout L(N, K);
-  if (n <= 16 || (L.KS <= ROW_WAVES && (long)((n + 15) / 16) * L.RT * L.KS <= 2000)) return {ROWS, 1, 0.};
+  if (n <= 16 || (L.KS <= ROW_WAVES && (long)((n + 15) / 16) * L.RT * L.KS <= 2000)) return {ROWS, 1, 4.};
   Choice best = {ROWS, 1, 1e30};
   for (int kind = 0; kind < KINDS; ++kind)
     for (int splits = 1; splits <= (kind < TILES ? 1 : 8); splits *= 2) {

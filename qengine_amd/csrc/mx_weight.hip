@@ -1,10 +1,10 @@
 // Weights in microscaled 4-bit floating point (E2M1 codes, a scale for 32 values): from bf16, and back.
 //
-// Both are bound by memory: 2 + 17/32 bytes a value. A wave owns 16 rows by 512 values: 4 KB of codes and 256 bytes
-// of scales, both contiguous. In bf16 a lane holds 8 neighbouring values, a quad a block, and 16 lanes a row's
+// Both are bound by memory: 2 + 17/32 bytes a value. A workgroup owns 16 rows by 512 values: 4 KB of codes and 256
+// bytes of scales, both contiguous. In bf16 a lane holds 8 neighbouring values, a quad a block, and 16 lanes a row's
 // 256 bytes, so that one instruction covers 4 rows by two whole lines; in codes a lane has 16 bytes, a block of one
 // row. A quad turns one into the other: lane q's dword of row 4 i + l is dword q of lane i, a 4 x 4 transposition.
-// 34816 x 5120: 87.5 us there, 84.5 us back, 5.2 and 5.3 TB/s, what a large copy reaches (with a block of 64 bytes a
+// 34816 x 5120: 80 us there, 79 us back, 5.7 TB/s, more than a large copy reaches (4.9; with a block of 64 bytes a
 // lane, whose instructions touch 64 lines each, 130 us).
 #include <limits.h>
 
@@ -29,13 +29,13 @@ __device__ __forceinline__ u32x4_t quad_transpose(u32x4_t d, int q) {
   return h ? u32x4_t{c, f, e2, e3} : u32x4_t{e0, e1, c, f};
 }
 
-// Where a wave is, and its lanes.
+// A workgroup has 16 rows by 512 values, a wave 128 of them.
 struct Place {
-  int rt, J, q, g, l;  // 16 rows, 512 values; quarter of a block, block of 128 values, row of four
+  int rt, J, t, q, g, l;  // 16 rows, 512 values, tile of 128; quarter of a block, block, row of four
   __device__ __forceinline__ Place(const Layout& L) {
-    const uint32_t id = blockIdx.x * 4 + threadIdx.x / WAVE;
-    rt = id / L.KS;
-    J = id % L.KS;
+    rt = blockIdx.x / L.KS;
+    J = blockIdx.x % L.KS;
+    t = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     q = threadIdx.x & 3;
     g = threadIdx.x >> 2 & 3;
     l = threadIdx.x >> 4 & 3;
@@ -45,94 +45,81 @@ struct Place {
 
 __global__ void __launch_bounds__(256)
 mx4_quant_kernel(const __bf16* __restrict__ w, long ldw, uint8_t* __restrict__ wq, int N, int K) {
+  __shared__ uint8_t scales[WAVE][4];
   const Layout L(N, K);
   const Place p(L);
-  if (p.rt >= L.RT) return;
-  u32x4_t v[4][4];  // of row 4 i + l, tile t
+  const int kt = p.J * 4 + p.t, k = kt * 128 + p.g * BLOCK + 8 * p.q;
+  u32x4_t v[4];  // of row 4 i + l
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int i = 0; i < 4; ++i) {
+    const int row = p.rt * 16 + 4 * i + p.l;
+    const __bf16* src = w + (size_t)row * ldw + k;
+    v[i] = u32x4_t{0u, 0u, 0u, 0u};
+    if (row < N && k + 8 <= K)
+      __builtin_memcpy(&v[i], src, 16);  // at any address
+    else if (row < N)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = p.rt * 16 + 4 * i + p.l, k = (p.J * 4 + t) * 128 + p.g * BLOCK + 8 * p.q;
-      const __bf16* src = w + (size_t)row * ldw + k;
-      v[t][i] = u32x4_t{0u, 0u, 0u, 0u};
-      if (row < N && k + 8 <= K)
-        __builtin_memcpy(&v[t][i], src, 16);  // at any address
-      else if (row < N)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (k + j < K) v[t][i][j / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(src)[j] << (16 * (j & 1));
-    }
-  uint32_t scales = 0;
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int kt = p.J * 4 + t;
-    if (kt >= L.KT) break;
-    u32x4_t codes;
-    uint32_t mine = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        top = max(top, max(v[t][i][j] << 16 & 0x7fffffffu, v[t][i][j] & 0x7fff0000u));
-      const int c = scale4(quad_max(top));
-      const float f = inverse(min(c, 253));
-      uint32_t d = 0;
-      d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, lo_bf16(v[t][i][0]) * f, hi_bf16(v[t][i][0]) * f, 1.0f, 0);
-      d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, lo_bf16(v[t][i][1]) * f, hi_bf16(v[t][i][1]) * f, 1.0f, 1);
-      d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, lo_bf16(v[t][i][2]) * f, hi_bf16(v[t][i][2]) * f, 1.0f, 2);
-      d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, lo_bf16(v[t][i][3]) * f, hi_bf16(v[t][i][3]) * f, 1.0f, 3);
-      codes[i] = c == 255 ? 0u : d;
-      mine = p.q == i ? (uint32_t)c : mine;
-    }
-    scales |= mine << (8 * t);
-    reinterpret_cast<u32x4_t*>(wq + ((size_t)p.rt * L.KT + kt) * 1024)[p.code_lane()] = quad_transpose(codes, p.q);
+      for (int j = 0; j < 8; ++j)
+        if (k + j < K) v[i][j / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(src)[j] << (16 * (j & 1));
   }
-  reinterpret_cast<uint32_t*>(wq + L.scales() + ((size_t)p.rt * L.KS + p.J) * 256)[p.code_lane()] = scales;
+  u32x4_t codes;
+  uint32_t mine = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = max(top, max(v[i][j] << 16 & 0x7fffffffu, v[i][j] & 0x7fff0000u));
+    const int c = scale4(quad_max(top));
+    const float f = inverse(min(c, 253));
+    uint32_t d = 0;
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, lo_bf16(v[i][0]) * f, hi_bf16(v[i][0]) * f, 1.0f, 0);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, lo_bf16(v[i][1]) * f, hi_bf16(v[i][1]) * f, 1.0f, 1);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, lo_bf16(v[i][2]) * f, hi_bf16(v[i][2]) * f, 1.0f, 2);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, lo_bf16(v[i][3]) * f, hi_bf16(v[i][3]) * f, 1.0f, 3);
+    codes[i] = c == 255 ? 0u : d;
+    mine = p.q == i ? (uint32_t)c : mine;
+  }
+  if (kt < L.KT)
+    reinterpret_cast<u32x4_t*>(wq + ((size_t)p.rt * L.KT + kt) * 1024)[p.code_lane()] = quad_transpose(codes, p.q);
+  scales[p.code_lane()][p.t] = kt < L.KT ? (uint8_t)mine : 0;
+  __syncthreads();
+  if (p.t == 0)
+    reinterpret_cast<uint32_t*>(wq + L.scales() + ((size_t)p.rt * L.KS + p.J) * 256)[threadIdx.x] =
+        reinterpret_cast<const uint32_t*>(scales)[threadIdx.x];
 }
 
 __global__ void __launch_bounds__(256)
 mx4_dequant_kernel(const uint8_t* __restrict__ wq, __bf16* __restrict__ out, long ldo, int N, int K) {
   const Layout L(N, K);
   const Place p(L);
-  if (p.rt >= L.RT) return;
-  const uint32_t scales =
-      reinterpret_cast<const uint32_t*>(wq + L.scales() + ((size_t)p.rt * L.KS + p.J) * 256)[p.code_lane()];
-  u32x4_t codes[4];
+  const int kt = p.J * 4 + p.t, k = kt * 128 + p.g * BLOCK + 8 * p.q;
+  if (kt >= L.KT) return;
+  const int scale = wq[L.scales() + ((size_t)p.rt * L.KS + p.J) * 256 + p.code_lane() * 4 + p.t];
+  const u32x4_t d =
+      quad_transpose(reinterpret_cast<const u32x4_t*>(wq + ((size_t)p.rt * L.KT + kt) * 1024)[p.code_lane()], p.q);
+  auto give = [&](int i, int c) {  // c: the scale of row 4 i + l
+    const float f = value(c);
+    // exact in fp32, and a bf16 value: a subnormal scale too
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d[i], 1.0f, 0);
+    const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d[i], 1.0f, 1);
+    const auto e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d[i], 1.0f, 2);
+    const auto h = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d[i], 1.0f, 3);
+    const u32x4_t v = {pack_bf16x2(a[0] * f, a[1] * f), pack_bf16x2(b[0] * f, b[1] * f),
+                       pack_bf16x2(e[0] * f, e[1] * f), pack_bf16x2(h[0] * f, h[1] * f)};
+    const int row = p.rt * 16 + 4 * i + p.l;
+    __bf16* dst = out + (size_t)row * ldo + k;
+    if (row < N && k + 8 <= K)
+      __builtin_memcpy(dst, &v, 16);  // at any address
+    else if (row < N)
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int kt = min(p.J * 4 + t, L.KT - 1);
-    codes[t] = reinterpret_cast<const u32x4_t*>(wq + ((size_t)p.rt * L.KT + kt) * 1024)[p.code_lane()];
-  }
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int k = (p.J * 4 + t) * 128 + p.g * BLOCK + 8 * p.q;
-    const u32x4_t d = quad_transpose(codes[t], p.q);
-    auto give = [&](int i, uint32_t all) {  // all: the scales of row 4 i + l
-      const float f = value((int)(all >> (8 * t) & 255u));
-      // exact in fp32, and a bf16 value: a subnormal scale too
-      const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d[i], 1.0f, 0);
-      const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d[i], 1.0f, 1);
-      const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d[i], 1.0f, 2);
-      const auto e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d[i], 1.0f, 3);
-      const u32x4_t v = {pack_bf16x2(a[0] * f, a[1] * f), pack_bf16x2(b[0] * f, b[1] * f),
-                         pack_bf16x2(c[0] * f, c[1] * f), pack_bf16x2(e[0] * f, e[1] * f)};
-      const int row = p.rt * 16 + 4 * i + p.l;
-      __bf16* dst = out + (size_t)row * ldo + k;
-      if (row < N && k + 8 <= K)
-        __builtin_memcpy(dst, &v, 16);  // at any address
-      else if (row < N)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (k + j < K) reinterpret_cast<uint16_t*>(dst)[j] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
-    };
-    // lane i of a quad has the scales of row 4 i + l
-    give(0, (uint32_t)__builtin_amdgcn_mov_dpp((int)scales, 0x00, 0xF, 0xF, false));
-    give(1, (uint32_t)__builtin_amdgcn_mov_dpp((int)scales, 0x55, 0xF, 0xF, false));
-    give(2, (uint32_t)__builtin_amdgcn_mov_dpp((int)scales, 0xAA, 0xF, 0xF, false));
-    give(3, (uint32_t)__builtin_amdgcn_mov_dpp((int)scales, 0xFF, 0xF, 0xF, false));
-  }
+      for (int j = 0; j < 8; ++j)
+        if (k + j < K) reinterpret_cast<uint16_t*>(dst)[j] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
+  };
+  // lane i of a quad has the scale of row 4 i + l
+  give(0, __builtin_amdgcn_mov_dpp(scale, 0x00, 0xF, 0xF, false));
+  give(1, __builtin_amdgcn_mov_dpp(scale, 0x55, 0xF, 0xF, false));
+  give(2, __builtin_amdgcn_mov_dpp(scale, 0xAA, 0xF, 0xF, false));
+  give(3, __builtin_amdgcn_mov_dpp(scale, 0xFF, 0xF, 0xF, false));
 }
 
 }  // namespace mx
@@ -143,9 +130,9 @@ using namespace qe::mx;
 
 extern "C" size_t qe_mx4_bytes(int N, int K) { return dims_ok(N, K) ? Layout(N, K).bytes() : 0; }
 
-// Workgroups of four waves, each with 16 rows by 512 values; 0 if more than a grid holds.
+// Workgroups; 0 if more than a grid holds.
 static uint32_t groups(const Layout& L) {
-  const size_t g = ((size_t)L.RT * L.KS + 3) / 4;
+  const size_t g = (size_t)L.RT * L.KS;
   return g <= UINT_MAX / 256 ? (uint32_t)g : 0;
 }
 
