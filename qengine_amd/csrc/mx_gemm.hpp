@@ -58,7 +58,7 @@ hipError_t gemm_tiles(TileKind kind, const Product& p, hipStream_t stream);
 
 // The kernels for some rows (mx_gemm_block.hip): tiles, and groups of waves that share K.
 enum class BlockKind { X64_W128, X64_W256, X32_W64_K4, COUNT };
-// K in parts of whole 512-value groups: 128-value tiles of a part, and the splits that hold any of K.
+// K in parts: 128-value tiles of one, and the splits that hold any of K.
 struct Parts {
   int part, splits;
 };

@@ -26,7 +26,7 @@ struct Block {
 
 struct BlockCall : Product {
   int xtiles, wtiles;
-  int part;  // 128-value tiles of a part of K, a multiple of 4
+  int part;  // 128-value tiles of a part of K
 };
 
 template <int WX, int WW, int WK, int TX, int TW, int STAGES, class T = Block<WX, WW, WK, TX, TW, STAGES>>
@@ -83,8 +83,9 @@ gemm_mx4_block_kernel(const BlockCall c) {
           (int)(wo[i] + min(wkt[i] + s, KT - 1) * 1024), 0, 0, 0);
   };
 
-  // scales of four tiles of K, as there
-  constexpr int SCALES = 2 * TW + TX;
+  // Scales of four steps. Of x, 16 bytes of lane r's row, the last ones shifted down from the row's end: no byte past
+  // the row is read, and blocks past K get code 0. Of the weight, dwords of four tiles each: a part begins within one.
+  constexpr int SCALES = 2 * TW + TX;  // loads of scales()
   const bool small = Kb < 16;
   const int last16 = small ? 0 : Kb - 16;
   const __amdgpu_buffer_rsrc_t sr = make_rsrc_uniform(c.wscale + (size_t)rt0 * L.KS * 256,
@@ -96,24 +97,31 @@ gemm_mx4_block_kernel(const BlockCall c) {
     xp[i] = c.xs + (size_t)min(x0 + (wx * TX + i) * 32 + r, c.n - 1) * c.lds;
     xp16[i] = small ? c.wq : xp[i];  // of no account where rows have fewer than 16 blocks
   }
-  uint32_t sw[TW][2], sw2[TW][2];
+  uint32_t sw[TW][2], sw0[TW][2], sw1[TW][2], sw2[TW][2];  // four steps' bytes; dwords at hand, the next, loaded
   u32x4_t sx[TX], sx2[TX];
-  auto scales = [&](int J) {
+  auto weight_scales = [&](int J) {
 #pragma unroll
     for (int j = 0; j < TW; ++j)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         sw2[j][h] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(
             sr, (int)(so + j * 2 * L.KS * 256 + min(J, L.KS - 1) * 256 + h * 128), 0, 0);
-#pragma unroll
-    for (int i = 0; i < TX; ++i) __builtin_memcpy(&sx2[i], xp16[i] + min(J * 16, last16), 16);
   };
-  auto take = [&](int J) {
-    const int cut = min(J * 16 - last16, 16);  // bytes
+  auto scales = [&](int k) {  // of tiles k .. k + 3
+    weight_scales(k / 4 + 1);
+#pragma unroll
+    for (int i = 0; i < TX; ++i) __builtin_memcpy(&sx2[i], xp16[i] + min(k * 4, last16), 16);
+  };
+  auto take = [&](int k) {
+    const int cut = min(k * 4 - last16, 16);  // bytes
 #pragma unroll
     for (int j = 0; j < TW; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) sw[j][h] = sw2[j][h];
+      for (int h = 0; h < 2; ++h) {
+        sw0[j][h] = sw1[j][h];
+        sw1[j][h] = sw2[j][h];
+        sw[j][h] = __builtin_amdgcn_alignbyte(sw1[j][h], sw0[j][h], k & 3);
+      }
     if (!small && cut > 0) {
 #pragma unroll
       for (int i = 0; i < TX; ++i) {
@@ -143,15 +151,20 @@ gemm_mx4_block_kernel(const BlockCall c) {
   const uint8_t* xf = smem + wk * T::PART + (wx * TX * 32 + r) * 128;
   const uint8_t* wf = smem + wk * T::PART + T::XB + (ww * TW * 2 + (r >> 4)) * 1024 + ((r & 15) + 16 * g) * 16;
 
-  scales(k0 / 4);
+  weight_scales(k0 / 4);
+#pragma unroll
+  for (int j = 0; j < TW; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) sw1[j][h] = sw2[j][h];
+  scales(k0);
   if (small) {
 #pragma unroll
     for (int i = 0; i < TX; ++i) {
       sx2[i] = u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const uint32_t v = xp[i][min(e, Kb - 1)];
-        sx2[i][e / 4] |= (e < Kb ? v : 0u) << (8 * (e & 3));
+        const uint32_t v = xp[i][min(k0 * 4 + e, Kb - 1)];
+        sx2[i][e / 4] |= (k0 * 4 + e < Kb ? v : 0u) << (8 * (e & 3));
       }
     }
   }
@@ -161,7 +174,7 @@ gemm_mx4_block_kernel(const BlockCall c) {
     fetch(s, s);
   }
   __builtin_amdgcn_sched_barrier(0);
-  take(k0 / 4);
+  take(k0);
   u32x4_t a[2][2][TW], b[2][2][TX][2];
   auto read = [&](int stage, int to) {
 #pragma unroll
@@ -184,15 +197,15 @@ gemm_mx4_block_kernel(const BlockCall c) {
   // A step, whose operands are in registers: the next step's are read behind the barrier (that stage has landed: only
   // the ST - 2 steps after it are out, and scales loaded since), the loads of the step ST ahead take the place of
   // this one, which every wave has read ahead of the barrier, and this step's products run meanwhile.
-#define QE_STEP(S)                                                                                            \
+#define QE_STEP(S, MORE)                                                                                      \
   {                                                                                                           \
-    vmcnt_wait<(T::ST - 2) * T::LOADS + (S >= 1 && S <= T::ST - 2 ? SCALES : 0)>();                           \
+    vmcnt_wait<(T::ST - 2) * T::LOADS + (MORE && S >= 1 && S <= T::ST - 2 ? SCALES : 0)>();                   \
     lds_barrier();                                                                                            \
     __builtin_amdgcn_sched_barrier(0);                                                                        \
     const int next = stage + 1 < T::ST ? stage + 1 : 0;                                                       \
     read(next, 1 - (S & 1));                                                                                  \
     __builtin_amdgcn_sched_barrier(0);                                                                        \
-    if (S == 0) scales((k0 + s0) / 4 + 1);                                                                    \
+    if (MORE && S == 0) scales(k0 + s0 + 4);                                                                  \
     __builtin_amdgcn_sched_barrier(0);                                                                        \
     fetch(s0 + S + T::ST, stage);                                                                             \
     __builtin_amdgcn_sched_barrier(0);                                                                        \
@@ -205,9 +218,15 @@ gemm_mx4_block_kernel(const BlockCall c) {
     __builtin_amdgcn_sched_barrier(0);                                                                        \
     stage = next;                                                                                             \
   }
-  for (int s0 = 0; s0 < c.part; s0 += 4) {
-    QE_STEP(0) QE_STEP(1) QE_STEP(2) QE_STEP(3)
-    take((k0 + s0) / 4 + 1);
+  int s0 = 0;
+  for (; s0 + 4 <= c.part; s0 += 4) {
+    QE_STEP(0, 1) QE_STEP(1, 1) QE_STEP(2, 1) QE_STEP(3, 1)
+    take(k0 + s0 + 4);
+  }
+  if (s0 < c.part) {  // the last one to three; no scales behind them
+    QE_STEP(0, 0)
+    if (s0 + 1 < c.part) { QE_STEP(1, 0) }
+    if (s0 + 2 < c.part) { QE_STEP(2, 0) }
   }
 #undef QE_STEP
   vmcnt_wait<0>();
@@ -265,8 +284,7 @@ mx4_sum_kernel(const float* ws, __bf16* out, long ldo, int n, int N, int width, 
 }
 
 static Parts parts(int wk, int K, int splits) {
-  const int KS = (K + 511) / 512, KT = (K + 127) / 128;
-  const int part = (KS + wk * splits - 1) / (wk * splits) * 4;
+  const int KT = (K + 127) / 128, part = (KT + wk * splits - 1) / (wk * splits);
   return {part, (KT + wk * part - 1) / (wk * part)};
 }
 

@@ -59,6 +59,39 @@ def test_product(native, n, N, K):
         C.check_product(out, xv, wv, K)
 
 
+@pytest.mark.parametrize("n,N", [(40, 3000), (100, 1100), (300, 4200), (500, 2300)])
+def test_every_remainder_of_k(native, n, N):
+    """Parts of K that begin and end anywhere: in groups of waves, in workgroups (with a workspace), in steps."""
+    import qengine_amd as qa
+    for blocks in (*range(4, 37), 70, 75, 131, 134, 193, 258, 261, 266, 330):
+        K = 32 * blocks
+        g = C.gen(n + K)
+        q, s, wq, xv, wv = case(native, g, n, N, K)
+        out = torch.full((n, N), float("nan"), dtype=BF, device=DEV)
+        ws = qa.alloc_mx4_ws(n, N, K).fill_(0xFF)
+        q, s = q.to(DEV), s.to(DEV)
+        native.gemm_mx4(wq, q, s, out, ws)
+        C.check_product(out, xv, wv, K)
+        first = out.clone()
+        for _ in range(3):
+            native.gemm_mx4(wq, q, s, out, ws)
+            assert torch.equal(first, out), K
+
+
+# weight rows past the last whole turn of the CUs go to another kernel: odd ends, strides, a workspace for them alone
+@pytest.mark.parametrize("n,N,K", [(200, 16501, 96), (100, 33003, 1000 // 32 * 32), (1000, 17000, 2048),
+                                   (70, 16900, 8192)])
+def test_wide_products(native, n, N, K):
+    import qengine_amd as qa
+    g = C.gen(N)
+    q, s, wq, xv, wv = case(native, g, n, N, K)
+    big = torch.full((n, N + 6), 7.0, dtype=BF, device=DEV)
+    for out in (big[:, 5: 5 + N], torch.empty(n, N, dtype=BF, device=DEV)):
+        native.gemm_mx4(wq, q.to(DEV), s.to(DEV), out, qa.alloc_mx4_ws(n, N, K).fill_(0xFF))
+        C.check_product(out, xv, wv, K)
+    assert (big[:, :5] == 7).all() and (big[:, 5 + N:] == 7).all()
+
+
 @pytest.mark.parametrize("n,N,K", [(1, 200, 96), (9, 200, 1056), (40, 200, 1056), (150, 200, 480), (600, 300, 480)])
 def test_nan_stays_in_its_row_and_column(native, n, N, K):
     g = C.gen(n)
