@@ -139,24 +139,24 @@ static hipError_t gemm_rows(const Product& c, hipStream_t stream) {
 // past the rule 25 x 13906 x 128 4.8 / 5.4, 55 x 15157 x 352 8.2 / 6.9, 17 x 5120 x 6144 9.6 / 7.8).
 // Between the others decides what each would take, in us: what a call costs at once, the steps of 128 of K of the
 // workgroups that take turns on a CU (a little longer while every CU has one), a workgroup's start and end, and outputs
-// (MB; a split writes and reads fp32 as well). The constants are least squares over 150 calls from 17 x 18 x 64 to
-// 2048 x 34816 x 5120, on which the choice is 4 % behind the best kernel and split (us, tiles of 256 x 256 /
-// 256 x 160 / 128 x 256 / 64 x 256 / 64 x 128 / 32 x 64): 2048 x 34816 x 5120 282 / 300 / 336 / - / 499 / 1215,
-// 2048 x 5120 x 6144 62 / 50 / 67 / - / 80 / 183, 1024 x 5120 x 5120 49 / 34 / 29 / 38 / 35 / 82,
-// 64 x 34816 x 5120 46 / 38 / 37 / 31 / 39 / 48 (272 tiles of 64 x 128 on 256 CUs, 136 of 64 x 256),
-// 300 x 5120 x 6144 53 / 38 / 32 / 20 / 15 / 27, 77 x 5001 x 6176 55 / 39 / 34 / 21 / 16 / 11. Splits:
-// 128 x 5120 x 17408 on 64 x 128, 48 us in one part, 22 in 2, 25 in 4; 40 x 100 x 17408 on 32 x 64, 17 in one, 9.0 in 4.
+// (MB; a split writes and reads fp32 as well). The constants are least squares over 120 calls from 17 x 80 x 64 to
+// 2048 x 34816 x 5120, on which the choice is 2 % behind the best kernel and split, 28 % at most (us, tiles of
+// 256 x 256 / 256 x 160 / 128 x 256 / 64 x 256 / 64 x 128 / 32 x 64): 2048 x 34816 x 5120
+// 281 / 295 / 326 / 425 / 491 / 1128, 2048 x 5120 x 6144 57 / 51 / 70 / 77 / 88 / 198, 1024 x 5120 x 5120
+// 46 / 33 / 29 / 39 / 37 / 80, 64 x 34816 x 5120 44 / 37 / 35 / 32 / 39 / 46 (272 tiles of 64 x 128 on 256 CUs, 136 of
+// 64 x 256), 300 x 5120 x 6144 53 / 37 / 31 / 22 / 15 / 27, 77 x 5001 x 6176 55 / 38 / 33 / 25 / 19 / 11. Splits:
+// 128 x 5120 x 17408 on 64 x 128, 48 us in one part, 31 in 2, 34 in 4; 40 x 100 x 17408 on 32 x 64, 16 in one, 9 in 4.
 struct Cost {
   int rows, cols;  // of a tile
   double call, step, full, group, split, out;
 };
 constexpr int TILES = (int)TileKind::COUNT, KINDS = TILES + (int)BlockKind::COUNT;
-static const Cost costs[KINDS] = {{256, 256, 10.5, 0.90, 0.09, 0.0, 0.0, 0.37},  // in TileKind's order
-                                  {128, 256, 8.5, 0.47, 0.18, 0.0, 0.0, 0.29},
-                                  {256, 160, 8.5, 0.59, 0.15, 0.0, 0.0, 0.34},
-                                  {64, 128, 4.1, 0.21, 0.04, 1.0, 1.8, 0.31},  // in BlockKind's
-                                  {64, 256, 3.9, 0.34, 0.06, 1.4, 2.1, 0.34},
-                                  {32, 64, 3.7, 0.39, 0.06, 1.8, 1.8, 0.28}};
+static const Cost costs[KINDS] = {{256, 256, 11.7, 0.91, 0.17, 0.0, 0.0, 0.22},  // in TileKind's order
+                                  {128, 256, 7.4, 0.53, 0.18, 0.0, 0.0, 0.26},
+                                  {256, 160, 8.1, 0.63, 0.19, 0.0, 0.0, 0.28},
+                                  {64, 128, 3.0, 0.25, 0.03, 1.2, 2.6, 0.32},  // in BlockKind's
+                                  {64, 256, 4.1, 0.37, 0.07, 2.0, 2.2, 0.35},
+                                  {32, 64, 2.4, 0.50, 0.00, 2.5, 2.6, 0.11}};
 
 constexpr int ROWS = -1;
 struct Choice {
@@ -198,7 +198,7 @@ static Choice choose(int n, int N, int K, size_t ws_bytes) {
 
 // A call, or two: the weight rows whose tiles give every CU the same number, and the others by what suits them (two
 // launches: by 3 % at least). 2048 x 34816 x 5120 is 1088 tiles of 256 x 256, 4.25 a CU: 282 us, with the last 2048
-// weight rows in 256 blocks of 64 x 256 271 us; 1024 x 34816 x 5120 163 and 142 us.
+// weight rows in 256 blocks of 64 x 256 274 us; 1024 x 34816 x 5120 165 and 139 us.
 struct Plan {
   Choice first, rest;
   int cut;  // weight rows of the first; N if that is all
