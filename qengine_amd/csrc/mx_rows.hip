@@ -3,7 +3,11 @@
 //
 // Vector forms give a lane 8 values (a 16-byte read, an 8-byte write), so a block is four neighbouring lanes and its
 // largest magnitude two lane moves; scalar forms, for widths or strides that are no multiple of 8, give a lane
-// one value and a block half a wave. Bound by memory; one row by the launch.
+// one value and a block half a wave. Bound by memory, one row by the launch: SwiGLU of 2048 x 17408 36 us (4.9 TB/s, a
+// large copy's rate), the norm of 2048 x 5120 14 us from the caches, 19 us from memory; of one row 2.7 us in a graph.
+// The norm's arithmetic is fp32, as in the framework's other norms: a value that lies within a few 2^-24 of the border
+// between two codes may get the other one (about 15 of 10.5 million). In 64 bits it would not, at 3.0 us for
+// one row and 20.5 us for 2048.
 #include "mx_common.hpp"
 
 namespace qe {
