@@ -1,13 +1,15 @@
 // Rows in microscaled 8-bit floating point (E4M3 codes, a scale for 32 values): of a norm with the residual's
 // addition, of SwiGLU, or of plain bf16 rows. The value is rounded once, from fp32 to its code.
 //
-// Vector forms give a lane 8 values (a 16-byte read, an 8-byte write), so a block is four neighbouring lanes and its
-// largest magnitude two lane moves; scalar forms, for widths or strides that are no multiple of 8, give a lane
-// one value and a block half a wave. Bound by memory, one row by the launch: SwiGLU of 2048 x 17408 36 us (4.9 TB/s, a
+// A lane has 8 values (a 16-byte read at any address, an 8-byte write), so a block is four neighbouring lanes and its
+// largest magnitude two lane moves. Bound by memory,
+// one row by the launch: SwiGLU of 2048 x 17408 36 us (4.9 TB/s, a
 // large copy's rate), the norm of 2048 x 5120 14 us from the caches, 19 us from memory; of one row 2.7 us in a graph.
 // The norm's arithmetic is fp32, as in the framework's other norms: a value that lies within a few 2^-24 of the border
 // between two codes may get the other one (about 15 of 10.5 million). In 64 bits it would not, at 3.0 us for
 // one row and 20.5 us for 2048.
+#include <algorithm>
+
 #include "mx_common.hpp"
 
 namespace qe {
@@ -19,6 +21,29 @@ __device__ __forceinline__ void unpack8(u32x4_t x, float (&v)[8]) {
     v[2 * i] = lo_bf16(x[i]);
     v[2 * i + 1] = hi_bf16(x[i]);
   }
+}
+
+// Values 8 c .. 8 c + 7 of a row of K, zeros from K on: the last ones come from the row's end, shifted down.
+__device__ __forceinline__ void load8(const __bf16* row, int c, int K, float (&v)[8]) {
+  u32x4_t x = {0u, 0u, 0u, 0u};
+  if (K >= 8) {
+    __builtin_memcpy(&x, row + min(8 * c, K - 8), 16);
+    const int cut = min(8 * c - (K - 8), 8);
+    if (cut > 0) {
+      uint64_t lo = (uint64_t)x[1] << 32 | x[0], hi = (uint64_t)x[3] << 32 | x[2];
+      if (cut >= 4) lo = hi, hi = 0;
+      if (cut >= 8) lo = 0;
+      const int bits = (cut & 3) * 16;
+      lo = lo >> bits | (bits ? hi << (64 - bits) : 0);
+      hi >>= bits;
+      x = u32x4_t{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 7; ++j)
+      if (8 * c + j < K) x[j / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[8 * c + j] << (16 * (j & 1));
+  }
+  unpack8(x, v);
 }
 
 // Eight values of this lane, a quarter of a block whose other quarters its three neighbours hold: codes and scale to
@@ -33,17 +58,6 @@ __device__ __forceinline__ void store8(const float (&v)[8], uint8_t* q, uint8_t*
   if ((c & 3) == 0) s[c >> 2] = (uint8_t)code;
 }
 
-// One value a lane, a block 32 lanes.
-__device__ __forceinline__ void store1(float v, uint8_t* q, uint8_t* s, int k, bool live) {
-  uint32_t top = magnitude(v);
-#pragma unroll
-  for (int o = 1; o < BLOCK; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-  const int code = scale8(top);
-  if (!live) return;
-  q[k] = code == 255 ? 0x7f : (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v * inverse(code), 0.f, 0, false) & 0xff);
-  if ((k & 31) == 0) s[k >> 5] = (uint8_t)code;
-}
-
 // silu(g) * u: exp and the reciprocal are the instructions' (1 ulp each), about 2^-22 relative in all, far below
 // the code's 2^-4.
 __device__ __forceinline__ float swiglu(float g, float u) {
@@ -51,34 +65,22 @@ __device__ __forceinline__ float swiglu(float g, float u) {
 }
 
 // ------------------------------------------------------------------------------ SwiGLU, plain rows
-template <bool GLU, bool VEC>
+template <bool GLU>
 __global__ void __launch_bounds__(256)
 act_mx8_kernel(const __bf16* __restrict__ x, long ldx, uint8_t* __restrict__ q, long ldq, uint8_t* __restrict__ s,
                long lds, int K) {
   const size_t r = blockIdx.x;
   const __bf16* xr = x + r * ldx;
-  uint8_t *qr = q + r * ldq, *sr = s + r * lds;
-  const int c = blockIdx.y * 256 + threadIdx.x, Kp = (K + BLOCK - 1) / BLOCK * BLOCK;
-  if constexpr (VEC) {
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c < K / 8) {
-      unpack8(reinterpret_cast<const u32x4_t*>(xr)[c], v);
-      if constexpr (GLU) {
-        float u[8];
-        unpack8(reinterpret_cast<const u32x4_t*>(xr + K)[c], u);
+  const int c = blockIdx.y * blockDim.x + threadIdx.x;
+  float v[8];
+  load8(xr, c, K, v);
+  if constexpr (GLU) {
+    float u[8];
+    load8(xr + K, c, K, u);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = swiglu(v[i], u[i]);
-      }
-    }
-    store8(v, qr, sr, c, c < Kp / 8);
-  } else {
-    float v = 0.f;
-    if (c < K) {
-      v = bf16_to_f32(xr[c]);
-      if constexpr (GLU) v = swiglu(v, bf16_to_f32(xr[K + c]));
-    }
-    store1(v, qr, sr, c, c < Kp);
+    for (int i = 0; i < 8; ++i) v[i] = swiglu(v[i], u[i]);
   }
+  store8(v, q + r * ldq, s + r * lds, c, c < (K + BLOCK - 1) / BLOCK * 4);
 }
 
 // ------------------------------------------------------------------------------ RMSNorm1p
@@ -95,78 +97,84 @@ __device__ __forceinline__ float sum_rows(float v, float* red) {
   return t;
 }
 
-// A workgroup a row, C pieces of 8 values a thread, all in registers: piece c of thread t is t + c * threads.
-template <int C>
-__global__ void __launch_bounds__(NORM_THREADS)
-norm_mx8_vec_kernel(const __bf16* __restrict__ x, long ldx, const __bf16* __restrict__ delta, long ldd,
-                    const __bf16* __restrict__ w, __bf16* __restrict__ sum, long ldsum, uint8_t* __restrict__ q,
-                    long ldq, uint8_t* __restrict__ s, long lds, int K, float eps) {
-  __shared__ float red[NORM_THREADS / WAVE];
-  const size_t r = blockIdx.x;
-  const int K8 = K / 8, P8 = (K + BLOCK - 1) / BLOCK * 4;
-  float v[C][8];
-  float ss = 0.f;
+// Piece c of a row, with delta added; the sum, rounded, is written and taken on with.
+__device__ __forceinline__ void load_sum(const __bf16* x, const __bf16* delta, __bf16* sum, int c, int K,
+                                         float (&v)[8]) {
+  load8(x, c, K, v);
+  if (!delta) return;
+  float d[8];
+  load8(delta, c, K, d);
+  u32x4_t o;
 #pragma unroll
-  for (int i = 0; i < C; ++i) {
-    const int c = threadIdx.x + i * blockDim.x;
+  for (int j = 0; j < 4; ++j) o[j] = pack_bf16x2(v[2 * j] + d[2 * j], v[2 * j + 1] + d[2 * j + 1]);
+  unpack8(o, v);
+  if (8 * c + 8 <= K) {
+    __builtin_memcpy(sum + 8 * c, &o, 16);
+  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    if (c < K8) {
-      unpack8(reinterpret_cast<const u32x4_t*>(x + r * ldx)[c], v[i]);
-      if (delta) {
-        float d[8];
-        unpack8(reinterpret_cast<const u32x4_t*>(delta + r * ldd)[c], d);
-        u32x4_t o;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          o[j] = pack_bf16x2(v[i][2 * j] + d[2 * j], v[i][2 * j + 1] + d[2 * j + 1]);
-          v[i][2 * j] = lo_bf16(o[j]);
-          v[i][2 * j + 1] = hi_bf16(o[j]);
-        }
-        reinterpret_cast<u32x4_t*>(sum + r * ldsum)[c] = o;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
-  }
-  const float inv = 1.0f / sqrtf(sum_rows(ss, red) / (float)K + eps);
-#pragma unroll
-  for (int i = 0; i < C; ++i) {
-    const int c = threadIdx.x + i * blockDim.x;
-    if (c < K8) {
-      float g[8];
-      unpack8(reinterpret_cast<const u32x4_t*>(w)[c], g);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = (v[i][j] * inv) * (1.0f + g[j]);
-    }
-    store8(v[i], q + r * ldq, s + r * lds, c, c < P8);
+    for (int j = 0; j < 7; ++j)
+      if (8 * c + j < K) reinterpret_cast<uint16_t*>(sum)[8 * c + j] = (uint16_t)(o[j / 2] >> (16 * (j & 1)));
   }
 }
 
-// Any width, stride and alignment: strided values, two passes over the row (the second reads what this thread read or
-// wrote, so no other thread's write is involved).
+__device__ __forceinline__ void weigh8(const __bf16* w, int c, int K, float inv, float (&v)[8]) {
+  float g[8];
+  load8(w, c, K, g);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (v[j] * inv) * (1.0f + g[j]);
+}
+
+__device__ __forceinline__ float squares(const float (&v)[8]) {
+  float t = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t += v[j] * v[j];
+  return t;
+}
+
+// A workgroup a row, C pieces of 8 values a thread, all in registers: piece c of thread t is t + c * threads.
+template <int C>
 __global__ void __launch_bounds__(NORM_THREADS)
 norm_mx8_kernel(const __bf16* x, long ldx, const __bf16* delta, long ldd, const __bf16* __restrict__ w, __bf16* sum,
                 long ldsum, uint8_t* __restrict__ q, long ldq, uint8_t* __restrict__ s, long lds, int K, float eps) {
   __shared__ float red[NORM_THREADS / WAVE];
   const size_t r = blockIdx.x;
-  const int Kp = (K + BLOCK - 1) / BLOCK * BLOCK;
+  float v[C][8];
   float ss = 0.f;
-  for (int c = threadIdx.x; c < K; c += blockDim.x) {
-    float v = bf16_to_f32(x[r * ldx + c]);
-    if (delta) {
-      const __bf16 b = f32_to_bf16(v + bf16_to_f32(delta[r * ldd + c]));
-      sum[r * ldsum + c] = b;
-      v = bf16_to_f32(b);
-    }
-    ss += v * v;
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    load_sum(x + r * ldx, delta ? delta + r * ldd : nullptr, sum + r * ldsum, threadIdx.x + i * blockDim.x, K, v[i]);
+    ss += squares(v[i]);
+  }
+  const float inv = 1.0f / sqrtf(sum_rows(ss, red) / (float)K + eps);
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    weigh8(w, c, K, inv, v[i]);
+    store8(v[i], q + r * ldq, s + r * lds, c, c < (K + BLOCK - 1) / BLOCK * 4);
+  }
+}
+
+// Rows that registers do not hold: two passes (the second reads what this thread read or wrote, so no other thread's
+// write is involved).
+__global__ void __launch_bounds__(NORM_THREADS)
+norm_mx8_wide_kernel(const __bf16* x, long ldx, const __bf16* delta, long ldd, const __bf16* __restrict__ w,
+                     __bf16* sum, long ldsum, uint8_t* __restrict__ q, long ldq, uint8_t* __restrict__ s, long lds,
+                     int K, float eps) {
+  __shared__ float red[NORM_THREADS / WAVE];
+  const size_t r = blockIdx.x;
+  const int pieces = (K + BLOCK - 1) / BLOCK * 4;
+  float v[8];
+  float ss = 0.f;
+  for (int c = threadIdx.x; c < pieces; c += blockDim.x) {
+    load_sum(x + r * ldx, delta ? delta + r * ldd : nullptr, sum + r * ldsum, c, K, v);
+    ss += squares(v);
   }
   const float inv = 1.0f / sqrtf(sum_rows(ss, red) / (float)K + eps);
   const __bf16* from = delta ? sum + r * ldsum : x + r * ldx;
-  // whole waves enter: a block's lanes meet in store1
-  for (int c = threadIdx.x; c - (int)(threadIdx.x & (WAVE - 1)) < Kp; c += blockDim.x) {
-    const float v = c < K ? (bf16_to_f32(from[c]) * inv) * (1.0f + bf16_to_f32(w[c])) : 0.f;
-    store1(v, q + r * ldq, s + r * lds, c, c < Kp);
+  for (int c = threadIdx.x; c < pieces; c += blockDim.x) {  // whole blocks enter: a multiple of four lanes
+    load8(from, c, K, v);
+    weigh8(w, c, K, inv, v);
+    store8(v, q + r * ldq, s + r * lds, c, true);
   }
 }
 
@@ -189,11 +197,10 @@ static hipError_t act(const void* x, long ldx, void* q, long ldq, void* s, long 
     return hipErrorInvalidValue;
   const auto* X = static_cast<const __bf16*>(x);
   auto *Q = static_cast<uint8_t*>(q), *S = static_cast<uint8_t*>(s);
-  const int Kp = (K + BLOCK - 1) / BLOCK * BLOCK;
-  if (K % 8 == 0 && ldx % 8 == 0 && aligned(x, 16))
-    act_mx8_kernel<GLU, true><<<dim3(n, (Kp / 8 + 255) / 256), dim3(256), 0, stream>>>(X, ldx, Q, ldq, S, lds, K);
-  else
-    act_mx8_kernel<GLU, false><<<dim3(n, (Kp + 255) / 256), dim3(256), 0, stream>>>(X, ldx, Q, ldq, S, lds, K);
+  const int pieces = (K + BLOCK - 1) / BLOCK * 4;
+  const int threads = std::min((pieces + WAVE - 1) / WAVE * WAVE, 256);
+  act_mx8_kernel<GLU><<<dim3(n, (pieces + threads - 1) / threads), dim3(threads), 0, stream>>>(X, ldx, Q, ldq, S,
+                                                                                               lds, K);
   return hipGetLastError();
 }
 
@@ -218,21 +225,15 @@ extern "C" hipError_t qe_rmsnorm1p_mx8(const void* x, long ldx, const void* delt
              *W = static_cast<const __bf16*>(w);
   auto* Sum = static_cast<__bf16*>(sum);
   auto *Q = static_cast<uint8_t*>(q), *S = static_cast<uint8_t*>(s);
-  const int P8 = (K + BLOCK - 1) / BLOCK * 4;
-  const bool vec = K % 8 == 0 && ldx % 8 == 0 && aligned(x, 16) && aligned(w, 16) && P8 <= 4 * NORM_THREADS &&
-                   (!delta || (ldd % 8 == 0 && ldsum % 8 == 0 && aligned(delta, 16) && aligned(sum, 16)));
+  const int pieces = (K + BLOCK - 1) / BLOCK * 4;
+  const int C = pieces <= NORM_THREADS ? 1 : pieces <= 2 * NORM_THREADS ? 2 : 4;
+  const int threads = std::min(((pieces + C - 1) / C + WAVE - 1) / WAVE * WAVE, NORM_THREADS);
 #define QE_NORM(...) \
   __VA_ARGS__<<<dim3(n), dim3(threads), 0, stream>>>(X, ldx, D, ldd, W, Sum, ldsum, Q, ldq, S, lds, K, eps)
-  if (vec) {
-    const int C = P8 <= NORM_THREADS ? 1 : P8 <= 2 * NORM_THREADS ? 2 : 4;
-    const int threads = ((P8 + C - 1) / C + WAVE - 1) / WAVE * WAVE;
-    if (C == 1) QE_NORM(norm_mx8_vec_kernel<1>);
-    else if (C == 2) QE_NORM(norm_mx8_vec_kernel<2>);
-    else QE_NORM(norm_mx8_vec_kernel<4>);
-  } else {
-    const int threads = K >= NORM_THREADS ? NORM_THREADS : (K + WAVE - 1) / WAVE * WAVE;
-    QE_NORM(norm_mx8_kernel);
-  }
+  if (C == 1) QE_NORM(norm_mx8_kernel<1>);
+  else if (C == 2) QE_NORM(norm_mx8_kernel<2>);
+  else if (pieces <= 4 * NORM_THREADS) QE_NORM(norm_mx8_kernel<4>);
+  else QE_NORM(norm_mx8_wide_kernel);
 #undef QE_NORM
   return hipGetLastError();
 }
