@@ -4,7 +4,8 @@
 // A lane has 8 values (a 16-byte read at any address, an 8-byte write), so a block is four neighbouring lanes and its
 // largest magnitude two lane moves. Bound by memory,
 // one row by the launch: SwiGLU of 2048 x 17408 36 us (4.9 TB/s, a
-// large copy's rate), the norm of 2048 x 5120 14 us from the caches, 19 us from memory; of one row 2.7 us in a graph.
+// large copy's rate), the norm of 2048 x 5120 14 us from the caches, 19 us from memory; of one row 2.7 us in a graph. Odd widths cost
+// 5 to 15 % more (value by value it was 2 to 3 times: 2048 x 5001 norm 52 us, 21.5 us so).
 // The norm's arithmetic is fp32, as in the framework's other norms: a value that lies within a few 2^-24 of the border
 // between two codes may get the other one (about 15 of 10.5 million). In 64 bits it would not, at 3.0 us for
 // one row and 20.5 us for 2048.
@@ -23,10 +24,12 @@ __device__ __forceinline__ void unpack8(u32x4_t x, float (&v)[8]) {
   }
 }
 
-// Values 8 c .. 8 c + 7 of a row of K, zeros from K on: the last ones come from the row's end, shifted down.
+// Values 8 c .. 8 c + 7 of a row of K, zeros from K on: the last ones come from the row's end, shifted down (TINY, K < 8:
+// value by value; a choice at run time would cost one row's norm 0.15 us of 2.7).
+template <bool TINY>
 __device__ __forceinline__ void load8(const __bf16* row, int c, int K, float (&v)[8]) {
   u32x4_t x = {0u, 0u, 0u, 0u};
-  if (K >= 8) {
+  if constexpr (!TINY) {
     __builtin_memcpy(&x, row + min(8 * c, K - 8), 16);
     const int cut = min(8 * c - (K - 8), 8);
     if (cut > 0) {
@@ -65,7 +68,7 @@ __device__ __forceinline__ float swiglu(float g, float u) {
 }
 
 // ------------------------------------------------------------------------------ SwiGLU, plain rows
-template <bool GLU>
+template <bool GLU, bool TINY>
 __global__ void __launch_bounds__(256)
 act_mx8_kernel(const __bf16* __restrict__ x, long ldx, uint8_t* __restrict__ q, long ldq, uint8_t* __restrict__ s,
                long lds, int K) {
@@ -73,10 +76,10 @@ act_mx8_kernel(const __bf16* __restrict__ x, long ldx, uint8_t* __restrict__ q, 
   const __bf16* xr = x + r * ldx;
   const int c = blockIdx.y * blockDim.x + threadIdx.x;
   float v[8];
-  load8(xr, c, K, v);
+  load8<TINY>(xr, c, K, v);
   if constexpr (GLU) {
     float u[8];
-    load8(xr + K, c, K, u);
+    load8<TINY>(xr + K, c, K, u);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = swiglu(v[i], u[i]);
   }
@@ -98,12 +101,13 @@ __device__ __forceinline__ float sum_rows(float v, float* red) {
 }
 
 // Piece c of a row, with delta added; the sum, rounded, is written and taken on with.
+template <bool TINY>
 __device__ __forceinline__ void load_sum(const __bf16* x, const __bf16* delta, __bf16* sum, int c, int K,
                                          float (&v)[8]) {
-  load8(x, c, K, v);
+  load8<TINY>(x, c, K, v);
   if (!delta) return;
   float d[8];
-  load8(delta, c, K, d);
+  load8<TINY>(delta, c, K, d);
   u32x4_t o;
 #pragma unroll
   for (int j = 0; j < 4; ++j) o[j] = pack_bf16x2(v[2 * j] + d[2 * j], v[2 * j + 1] + d[2 * j + 1]);
@@ -117,9 +121,10 @@ __device__ __forceinline__ void load_sum(const __bf16* x, const __bf16* delta, _
   }
 }
 
+template <bool TINY>
 __device__ __forceinline__ void weigh8(const __bf16* w, int c, int K, float inv, float (&v)[8]) {
   float g[8];
-  load8(w, c, K, g);
+  load8<TINY>(w, c, K, g);
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = (v[j] * inv) * (1.0f + g[j]);
 }
@@ -132,7 +137,7 @@ __device__ __forceinline__ float squares(const float (&v)[8]) {
 }
 
 // A workgroup a row, C pieces of 8 values a thread, all in registers: piece c of thread t is t + c * threads.
-template <int C>
+template <int C, bool TINY>
 __global__ void __launch_bounds__(NORM_THREADS)
 norm_mx8_kernel(const __bf16* x, long ldx, const __bf16* delta, long ldd, const __bf16* __restrict__ w, __bf16* sum,
                 long ldsum, uint8_t* __restrict__ q, long ldq, uint8_t* __restrict__ s, long lds, int K, float eps) {
@@ -142,14 +147,14 @@ norm_mx8_kernel(const __bf16* x, long ldx, const __bf16* delta, long ldd, const 
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    load_sum(x + r * ldx, delta ? delta + r * ldd : nullptr, sum + r * ldsum, threadIdx.x + i * blockDim.x, K, v[i]);
+    load_sum<TINY>(x + r * ldx, delta ? delta + r * ldd : nullptr, sum + r * ldsum, threadIdx.x + i * blockDim.x, K, v[i]);
     ss += squares(v[i]);
   }
   const float inv = 1.0f / sqrtf(sum_rows(ss, red) / (float)K + eps);
 #pragma unroll
   for (int i = 0; i < C; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
-    weigh8(w, c, K, inv, v[i]);
+    weigh8<TINY>(w, c, K, inv, v[i]);
     store8(v[i], q + r * ldq, s + r * lds, c, c < (K + BLOCK - 1) / BLOCK * 4);
   }
 }
@@ -166,14 +171,14 @@ norm_mx8_wide_kernel(const __bf16* x, long ldx, const __bf16* delta, long ldd, c
   float v[8];
   float ss = 0.f;
   for (int c = threadIdx.x; c < pieces; c += blockDim.x) {
-    load_sum(x + r * ldx, delta ? delta + r * ldd : nullptr, sum + r * ldsum, c, K, v);
+    load_sum<false>(x + r * ldx, delta ? delta + r * ldd : nullptr, sum + r * ldsum, c, K, v);
     ss += squares(v);
   }
   const float inv = 1.0f / sqrtf(sum_rows(ss, red) / (float)K + eps);
   const __bf16* from = delta ? sum + r * ldsum : x + r * ldx;
   for (int c = threadIdx.x; c < pieces; c += blockDim.x) {  // whole blocks enter: a multiple of four lanes
-    load8(from, c, K, v);
-    weigh8(w, c, K, inv, v);
+    load8<false>(from, c, K, v);
+    weigh8<false>(w, c, K, inv, v);
     store8(v, q + r * ldq, s + r * lds, c, true);
   }
 }
@@ -199,8 +204,11 @@ static hipError_t act(const void* x, long ldx, void* q, long ldq, void* s, long 
   auto *Q = static_cast<uint8_t*>(q), *S = static_cast<uint8_t*>(s);
   const int pieces = (K + BLOCK - 1) / BLOCK * 4;
   const int threads = std::min((pieces + WAVE - 1) / WAVE * WAVE, 256);
-  act_mx8_kernel<GLU><<<dim3(n, (pieces + threads - 1) / threads), dim3(threads), 0, stream>>>(X, ldx, Q, ldq, S,
-                                                                                               lds, K);
+  const dim3 grid(n, (pieces + threads - 1) / threads);
+  if (K >= 8)
+    act_mx8_kernel<GLU, false><<<grid, dim3(threads), 0, stream>>>(X, ldx, Q, ldq, S, lds, K);
+  else
+    act_mx8_kernel<GLU, true><<<grid, dim3(threads), 0, stream>>>(X, ldx, Q, ldq, S, lds, K);
   return hipGetLastError();
 }
 
@@ -230,9 +238,10 @@ extern "C" hipError_t qe_rmsnorm1p_mx8(const void* x, long ldx, const void* delt
   const int threads = std::min(((pieces + C - 1) / C + WAVE - 1) / WAVE * WAVE, NORM_THREADS);
 #define QE_NORM(...) \
   __VA_ARGS__<<<dim3(n), dim3(threads), 0, stream>>>(X, ldx, D, ldd, W, Sum, ldsum, Q, ldq, S, lds, K, eps)
-  if (C == 1) QE_NORM(norm_mx8_kernel<1>);
-  else if (C == 2) QE_NORM(norm_mx8_kernel<2>);
-  else if (pieces <= 4 * NORM_THREADS) QE_NORM(norm_mx8_kernel<4>);
+  if (K < 8) QE_NORM(norm_mx8_kernel<1, true>);
+  else if (C == 1) QE_NORM(norm_mx8_kernel<1, false>);
+  else if (C == 2) QE_NORM(norm_mx8_kernel<2, false>);
+  else if (pieces <= 4 * NORM_THREADS) QE_NORM(norm_mx8_kernel<4, false>);
   else QE_NORM(norm_mx8_wide_kernel);
 #undef QE_NORM
   return hipGetLastError();
