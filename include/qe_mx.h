@@ -54,8 +54,11 @@ hipError_t qe_rmsnorm1p_mx8(const void* x, long ldx, const void* delta, long ldd
 /* out[r][j] = bf16(sum over k of x[r][k] * w[j][k]), x the values of the mx8 rows xq [n][ldx], xs [n][lds] and w
  * those of wq (mx4 of [N][K]), products and sums in fp32. K is a multiple of 32 (the width of xq). out [n][ldo]
  * bf16. A NaN of x[r] reaches every out[r][j].
+ * Up to 16 rows: row r has the bits of a 1-row call. More rows: the order of a row's sums follows from n, N, K and
+ * the workspace's size (the same call gives the same bits).
  * ws: qe_gemm_mx4_ws_size(n, N, K) bytes, 16-byte aligned, any contents, one per call in flight (NULL where that
- * is 0; with fewer bytes the call runs without it, in another order of sums).
+ * is 0; with fewer bytes the call runs without it, in another order of sums). Graphs that share one must not be
+ * replayed at the same time.
  * Valid: n >= 1, N >= 1, K >= 32, ldx >= K and a multiple of 16, xq and wq 16-byte aligned, lds >= K / 32,
  * ldo >= N. */
 hipError_t qe_gemm_mx4(const void* wq, const void* xq, long ldx, const void* xs, long lds, void* out, long ldo,

@@ -29,6 +29,10 @@ Parity status per function (each is pinned by checks in ``tests/test_oracle.py``
                                                       -> pinned (the contiguous oracle over gathered
                                                          pages, brute force, closed forms;
                                                          tests/test_paged_oracle.py)
+  mx_oracle: quant4 / quant8, values, product, swiglu, rmsnorm1p
+                                                      -> pinned (every code and scale by search, torch's
+                                                         float8_e4m3fn, closed forms;
+                                                         tests/test_mx_oracle.py)
 """
 from .attn_oracle import *  # noqa: F401,F403
 from .gemv_oracle import gemv_bf16_ref, gemv_bound, gemv_exact  # noqa: F401

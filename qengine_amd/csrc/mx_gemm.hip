@@ -13,9 +13,12 @@ namespace qe {
 namespace mx {
 
 // ------------------------------------------------------------------------------ up to 16 rows
-// Streams the weight. A workgroup takes MT tiles of 16 weight rows; its waves, as many as K has groups of 512 values, or
-// a whole fraction of that (at most 16), share K by groups and their sums are added in order. A column of the product is one
-// row of x, which no other column touches, and the split goes by K alone: a row's bits do not depend on the others.
+// Streams the weight: bound by memory. A workgroup takes MT tiles of 16 weight rows; its waves, as many as K has
+// groups of 512 values, or a whole fraction of that (at most 16), share K by groups and their sums are added in order.
+// A wave loads a whole group (MT 4 KB of codes) before it multiplies, so that a CU has up to 128 KB on the way. A
+// column of the product is one row of x, which no other column touches, and the split goes by K alone: a row's bits
+// do not depend on the others. 1 x 14336 x 5120 8.6 us (39 MB, 4.5 TB/s; a copy reaches 4.9), 1 x 34816 x 5120
+// 18.6 us, 5 x 5120 x 17408 12.2 us (160 workgroups; 47 MB).
 constexpr int ROW_WAVES = 16;
 
 template <int MT, bool ONE>
@@ -113,6 +116,9 @@ gemm_mx4_rows_kernel(const Product c, int per) {
   }
 }
 
+// Tiles of a workgroup: two, so that a row of x is read half as often, while that leaves as many workgroups as 5/8 of
+// the CUs; four where x has more rows than the loads of two hide (us of 1 / 2 / 4: 1 x 5120 x 17408 13.5 / 12.3 /
+// 20.7, 3 x 1393 x 1472 4.0 / 4.1 / 4.9, 16 x 34816 x 5120 31.8 / 25.2 / 24.9, 16 x 14336 x 5120 - / 11.2 / 10.0).
 static hipError_t gemm_rows(const Product& c, hipStream_t stream) {
   const Layout L(c.N, c.K);
   const int per = (L.KS + ROW_WAVES - 1) / ROW_WAVES, waves = (L.KS + per - 1) / per, xt = (c.n + 15) / 16;
@@ -137,15 +143,21 @@ static hipError_t gemm_rows(const Product& c, hipStream_t stream) {
 // Up to 16 rows always go to the streaming kernel, or a row's bits would depend on the others. More rows do where the
 // work is small and K short (us, it / the best of the others: 32 x 1000 x 1000 3.9 / 5.6, 102 x 171 x 2176 4.6 / 6.8;
 // past the rule 25 x 13906 x 128 4.8 / 5.4, 55 x 15157 x 352 8.2 / 6.9, 17 x 5120 x 6144 9.6 / 7.8).
+//
 // Between the others decides what each would take, in us: what a call costs at once, the steps of 128 of K of the
-// workgroups that take turns on a CU (a little longer while every CU has one), a workgroup's start and end, and outputs
-// (MB; a split writes and reads fp32 as well). The constants are least squares over 120 calls from 17 x 80 x 64 to
-// 2048 x 34816 x 5120, on which the choice is 2 % behind the best kernel and split, 28 % at most (us, tiles of
-// 256 x 256 / 256 x 160 / 128 x 256 / 64 x 256 / 64 x 128 / 32 x 64): 2048 x 34816 x 5120
-// 281 / 295 / 326 / 425 / 491 / 1128, 2048 x 5120 x 6144 57 / 51 / 70 / 77 / 88 / 198, 1024 x 5120 x 5120
-// 46 / 33 / 29 / 39 / 37 / 80, 64 x 34816 x 5120 44 / 37 / 35 / 32 / 39 / 46 (272 tiles of 64 x 128 on 256 CUs, 136 of
-// 64 x 256), 300 x 5120 x 6144 53 / 37 / 31 / 22 / 15 / 27, 77 x 5001 x 6176 55 / 38 / 33 / 25 / 19 / 11. Splits:
-// 128 x 5120 x 17408 on 64 x 128, 48 us in one part, 31 in 2, 34 in 4; 40 x 100 x 17408 on 32 x 64, 16 in one, 9 in 4.
+// workgroups that take turns on a CU (a little longer while every CU has one), a workgroup's start and end, and
+// outputs (MB; a split writes and reads fp32 as well). The constants are least squares over 120 calls from
+// 17 x 80 x 64 to 2048 x 34816 x 5120, on which the choice is 2 % behind the best kernel and split, 15 % at most. us,
+// tiles of 256 x 256 / 256 x 160 / 128 x 256 / 64 x 256 / 64 x 128 / 32 x 128 / 32 x 64:
+//   2048 x 34816 x 5120  281 / 295 / 326 / 425 / 491 / - / 1128
+//   2048 x 5120 x 6144   57 / 51 / 70 / 77 / 88 / - / 198
+//   1024 x 5120 x 5120   46 / 33 / 29 / 39 / 37 / - / 80
+//   64 x 34816 x 5120    44 / 37 / 35 / 32 / 39 / 41 / 46 (272 tiles of 64 x 128 on 256 CUs, 136 of 64 x 256)
+//   300 x 5120 x 6144    53 / 37 / 31 / 22 / 15 / 20 / 27
+//   687 x 1326 x 5056    - / - / - / - / 15.8 / 12.6 / -
+//   77 x 5001 x 6176     55 / 38 / 33 / 25 / 19 / 13.6 / 10.7
+// Splits: 128 x 5120 x 17408 on 64 x 128, 48 us in one part, 31 in 2, 34 in 4; 40 x 100 x 17408 on 32 x 64, 16 in one, 9
+// in 4.
 struct Cost {
   int rows, cols;  // of a tile
   double call, step, full, group, split, out;
@@ -156,6 +168,7 @@ static const Cost costs[KINDS] = {{256, 256, 11.7, 0.91, 0.17, 0.0, 0.0, 0.22}, 
                                   {256, 160, 8.1, 0.63, 0.19, 0.0, 0.0, 0.28},
                                   {64, 128, 3.0, 0.25, 0.03, 1.2, 2.6, 0.32},  // in BlockKind's
                                   {64, 256, 4.1, 0.37, 0.07, 2.0, 2.2, 0.35},
+                                  {32, 128, 2.7, 0.34, 0.03, 2.6, 2.6, 0.20},
                                   {32, 64, 2.4, 0.50, 0.00, 2.5, 2.6, 0.11}};
 
 constexpr int ROWS = -1;
@@ -172,7 +185,8 @@ static long tiles(const Cost& c, int n, int N) {
 static double estimate(int kind, int splits, int n, int N, int K) {
   const Cost& c = costs[kind];
   const double cus = compute_units(), turns = (double)tiles(c, n, N) * splits / cus, mb = 2e-6 * n * N;
-  const int steps = kind < TILES ? std::max((K + 127) / 128, 2) : block_parts((BlockKind)(kind - TILES), K, splits).part;
+  const int steps =
+      kind < TILES ? std::max((K + 127) / 128, 2) : block_parts((BlockKind)(kind - TILES), K, splits).part;
   return c.call + std::ceil(turns) * steps * (c.step + c.full * std::min(turns, 1.)) + turns * c.group +
          (splits > 1 ? c.split + c.out * mb * (2 * splits + 1) : c.out * mb);
 }

@@ -1,5 +1,11 @@
 // The product of 8-bit rows and a 4-bit weight for tens to hundreds of rows: small tiles, K shared by groups of waves
 // and, where there are few tiles, by workgroups.
+//
+// Bound by what a CU takes in: about 60 GB/s of lines that its L2 has to fetch, 90 of others, however many loads are
+// on the way (four or eight steps ahead, the weight through LDS or into registers, K begun elsewhere by every
+// workgroup: all the same), so that a tile's bytes a step decide: x 128 ROWS + w 64 COLS. 300 x 5120 x 6144 is 200
+// tiles of 64 x 128, 48 steps of 16 KB: 14.6 us, 1,290 TFLOP/s; 77 x 5001 x 6176 237 tiles of 32 x 64 whose four
+// parts of K run side by side, 13 steps of 32 KB: 10.7 us; 64 x 34816 x 5120 32 us.
 #include <limits.h>
 
 #include <algorithm>
@@ -37,16 +43,16 @@ gemm_mx4_block_kernel(const BlockCall c) {
   const int lane = threadIdx.x & (WAVE - 1), r = lane & 31, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int wx = w % WX, ww = w / WX % WW, wk = w / (WX * WW);
-  // workgroups go to the 8 XCDs in turn: each gets neighbouring tiles, the row tiles of a weight tile first, so that the
-  // weight is read by one L2
+  // workgroups go to the 8 XCDs in turn: each gets neighbouring tiles, the row tiles of a weight tile first, so that
+  // the weight is read by one L2
   const int tiles = c.xtiles * c.wtiles, q8 = tiles / 8, r8 = tiles % 8, xcd = blockIdx.x % 8;
   const int tile = xcd * q8 + min(xcd, r8) + (int)blockIdx.x / 8;
   const int x0 = tile % c.xtiles * T::ROWS, c0 = tile / c.xtiles * T::COLS, rt0 = c0 / 16;
   const int KT = L.KT, Kb = c.K / BLOCK;
   const int k0 = (blockIdx.y * WK + wk) * c.part;  // this wave's first tile of K
 
-  // loads: as in the kernel for many rows, pieces of x (8 rows of 128 bytes, slot s of row i holds chunk s ^ (i / 2 % 8))
-  // and of the weight (a 16-row tile's 1 KB) of every part
+  // loads: as in the kernel for many rows, pieces of x (8 rows of 128 bytes, slot s of row i holds chunk s ^ (i / 2 %
+  // 8)) and of the weight (a 16-row tile's 1 KB) of every part
   const __amdgpu_buffer_rsrc_t xr =
       make_rsrc_uniform(c.xq + (size_t)x0 * c.ldx, (uint32_t)((size_t)(min(T::ROWS, c.n - x0) - 1) * c.ldx + c.K));
   const __amdgpu_buffer_rsrc_t wr = make_rsrc_uniform(c.wq + (size_t)rt0 * KT * 1024,
@@ -305,13 +311,14 @@ static hipError_t run(const Product& p, int splits, hipStream_t stream) {
 }
 
 Parts block_parts(BlockKind kind, int K, int splits) {
-  return parts(kind == BlockKind::X32_W64_K4 ? 4 : 1, K, splits);
+  return parts(kind == BlockKind::X32_W64_K4 ? 4 : kind == BlockKind::X32_W128_K2 ? 2 : 1, K, splits);
 }
 
 hipError_t gemm_blocks(BlockKind kind, int splits, const Product& p, hipStream_t stream) {
   switch (kind) {
     case BlockKind::X64_W128: return run<2, 4, 1, 1, 1, 4>(p, splits, stream);
     case BlockKind::X64_W256: return run<2, 4, 1, 1, 2, 4>(p, splits, stream);
+    case BlockKind::X32_W128_K2: return run<1, 4, 2, 1, 1, 4>(p, splits, stream);
     case BlockKind::X32_W64_K4: return run<1, 2, 4, 1, 1, 3>(p, splits, stream);
     default: return hipErrorInvalidValue;
   }

@@ -2,13 +2,12 @@
 // addition, of SwiGLU, or of plain bf16 rows. The value is rounded once, from fp32 to its code.
 //
 // A lane has 8 values (a 16-byte read at any address, an 8-byte write), so a block is four neighbouring lanes and its
-// largest magnitude two lane moves. Bound by memory,
-// one row by the launch: SwiGLU of 2048 x 17408 36 us (4.9 TB/s, a
-// large copy's rate), the norm of 2048 x 5120 14 us from the caches, 19 us from memory; of one row 2.7 us in a graph. Odd widths cost
-// 5 to 15 % more (value by value it was 2 to 3 times: 2048 x 5001 norm 52 us, 21.5 us so).
-// The norm's arithmetic is fp32, as in the framework's other norms: a value that lies within a few 2^-24 of the border
-// between two codes may get the other one (about 15 of 10.5 million). In 64 bits it would not, at 3.0 us for
-// one row and 20.5 us for 2048.
+// largest magnitude two lane moves. Bound by memory, one row by the launch: SwiGLU of 2048 x 17408 36 us (4.9 TB/s, a
+// large copy's rate), the norm of 2048 x 5120 14 us from the caches, 19 us from memory; of one row 2.7 us in a graph.
+// Odd widths cost 5 to 15 % more (value by value it was 2 to 3 times: 2048 x 5001 norm 52 us, 21.5 us so). The norm's
+// arithmetic is fp32, as in the framework's other norms: a value that lies within a few 2^-24 of the border between
+// two codes may get the other one (about 15 of 10.5 million). In 64 bits it would not, at 3.0 us for one row and 20.5
+// us for 2048.
 #include <algorithm>
 
 #include "mx_common.hpp"
@@ -24,8 +23,8 @@ __device__ __forceinline__ void unpack8(u32x4_t x, float (&v)[8]) {
   }
 }
 
-// Values 8 c .. 8 c + 7 of a row of K, zeros from K on: the last ones come from the row's end, shifted down (TINY, K < 8:
-// value by value; a choice at run time would cost one row's norm 0.15 us of 2.7).
+// Values 8 c .. 8 c + 7 of a row of K, zeros from K on: the last ones come from the row's end, shifted down (TINY, K
+// < 8: value by value; a choice at run time would cost one row's norm 0.15 us of 2.7).
 template <bool TINY>
 __device__ __forceinline__ void load8(const __bf16* row, int c, int K, float (&v)[8]) {
   u32x4_t x = {0u, 0u, 0u, 0u};
@@ -147,7 +146,8 @@ norm_mx8_kernel(const __bf16* x, long ldx, const __bf16* delta, long ldd, const 
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    load_sum<TINY>(x + r * ldx, delta ? delta + r * ldd : nullptr, sum + r * ldsum, threadIdx.x + i * blockDim.x, K, v[i]);
+    load_sum<TINY>(x + r * ldx, delta ? delta + r * ldd : nullptr, sum + r * ldsum, threadIdx.x + i * blockDim.x, K,
+                   v[i]);
     ss += squares(v[i]);
   }
   const float inv = 1.0f / sqrtf(sum_rows(ss, red) / (float)K + eps);
