@@ -196,3 +196,42 @@ def test_offsets_past_32_bits(native):
     native.gemm_mx4(wq, qd, sd, out)
     C.check_product(out[-5:], M.values8(q, s), wv, K)
     assert (out[: n - 5] == 0).all()
+
+
+@pytest.mark.parametrize("n,N,K", [(100, 513, 17408), (40, 100, 9376)])
+def test_workspaces_of_any_size(native, n, N, K):
+    """A workspace that is too small for a split is used for a smaller one, or not at all; no byte past it is written."""
+    import qengine_amd as qa
+    g = C.gen(n)
+    q, s, wq, xv, wv = case(native, g, n, N, K)
+    need = qa.mx4_ws_bytes(n, N, K)
+    assert need > 0
+    out = torch.empty(n, N, dtype=BF, device=DEV)
+    for size in (need + 4096, need, need - 16, need // 2, need // 4 // 16 * 16, 16, 0):
+        big = torch.full((size + 65536,), 0x55, dtype=U8, device=DEV)
+        out.fill_(float("nan"))
+        native.gemm_mx4(wq, q.to(DEV), s.to(DEV), out, big[:size])
+        C.check_product(out, xv, wv, K)
+        assert (big[max(size, 0):] == 0x55).all(), size
+
+
+def test_weights_past_32_bits(native):
+    """Codes of a weight that lie past 2^32 bytes: quantised, read back, and multiplied by one row and by many."""
+    import qengine_amd as qa
+    N, K, m = 270016, 32768, 40
+    w = torch.zeros(N, K, dtype=BF, device=DEV)  # 17.7 GB, 4.4 GB of codes
+    g = C.gen(3)
+    tail = (torch.randn(m, K, generator=g) * K ** -0.5).to(BF)
+    w[-m:].copy_(tail)
+    wq = qa.alloc_mx4(N, K, DEV)
+    native.mx4_quant(w, wq)
+    native.mx4_dequant(wq, w.fill_(1.0))
+    want = M.values4(*M.quant4(tail))
+    assert torch.equal(w[-m:].cpu().to(F64), want.to(F64)) and not w[:-m:4096].any()
+    del w
+    for n in (1, 20, 300):
+        q, s = rows8(g, n, K)
+        out = torch.empty(n, N, dtype=BF, device=DEV)
+        native.gemm_mx4(wq, q.to(DEV), s.to(DEV), out)
+        C.check_product(out[:, -m:].contiguous(), M.values8(q, s), want, K)
+        assert not out[:, :-m].any(), n
