@@ -189,6 +189,8 @@ norm_mx8_wide_kernel(const __bf16* x, long ldx, const __bf16* delta, long ldd, c
 using namespace qe;
 using namespace qe::mx;
 
+constexpr int LAUNCH_ROWS = 1 << 21;  // a grid has fewer than 2^32 threads
+
 static bool rows_ok(const void* q, long ldq, const void* s, long lds, int n, int K) {
   const long blocks = (K + BLOCK - 1) / BLOCK;
   return q && s && dims_ok(n, K) && ld_ok(ldq, blocks * BLOCK) && ldq % 16 == 0 && aligned(q, 16) &&
@@ -204,11 +206,15 @@ static hipError_t act(const void* x, long ldx, void* q, long ldq, void* s, long 
   auto *Q = static_cast<uint8_t*>(q), *S = static_cast<uint8_t*>(s);
   const int pieces = (K + BLOCK - 1) / BLOCK * 4;
   const int threads = std::min((pieces + WAVE - 1) / WAVE * WAVE, 256);
-  const dim3 grid(n, (pieces + threads - 1) / threads);
-  if (K >= 8)
-    act_mx8_kernel<GLU, false><<<grid, dim3(threads), 0, stream>>>(X, ldx, Q, ldq, S, lds, K);
-  else
-    act_mx8_kernel<GLU, true><<<grid, dim3(threads), 0, stream>>>(X, ldx, Q, ldq, S, lds, K);
+  for (int r = 0; r < n; r += LAUNCH_ROWS) {
+    const dim3 grid(std::min(n - r, LAUNCH_ROWS), (pieces + threads - 1) / threads);
+    if (K >= 8)
+      act_mx8_kernel<GLU, false><<<grid, dim3(threads), 0, stream>>>(X + r * ldx, ldx, Q + r * ldq, ldq, S + r * lds,
+                                                                     lds, K);
+    else
+      act_mx8_kernel<GLU, true><<<grid, dim3(threads), 0, stream>>>(X + r * ldx, ldx, Q + r * ldq, ldq, S + r * lds,
+                                                                    lds, K);
+  }
   return hipGetLastError();
 }
 
@@ -236,13 +242,19 @@ extern "C" hipError_t qe_rmsnorm1p_mx8(const void* x, long ldx, const void* delt
   const int pieces = (K + BLOCK - 1) / BLOCK * 4;
   const int C = pieces <= NORM_THREADS ? 1 : pieces <= 2 * NORM_THREADS ? 2 : 4;
   const int threads = std::min(((pieces + C - 1) / C + WAVE - 1) / WAVE * WAVE, NORM_THREADS);
-#define QE_NORM(...) \
-  __VA_ARGS__<<<dim3(n), dim3(threads), 0, stream>>>(X, ldx, D, ldd, W, Sum, ldsum, Q, ldq, S, lds, K, eps)
-  if (K < 8) QE_NORM(norm_mx8_kernel<1, true>);
-  else if (C == 1) QE_NORM(norm_mx8_kernel<1, false>);
-  else if (C == 2) QE_NORM(norm_mx8_kernel<2, false>);
-  else if (pieces <= 4 * NORM_THREADS) QE_NORM(norm_mx8_kernel<4, false>);
-  else QE_NORM(norm_mx8_wide_kernel);
+  for (int r = 0; r < n; r += LAUNCH_ROWS) {
+    const __bf16* d = D ? D + r * ldd : nullptr;
+    __bf16* to = Sum ? Sum + r * ldsum : nullptr;
+#define QE_NORM(...)                                                                                              \
+  __VA_ARGS__<<<dim3(std::min(n - r, LAUNCH_ROWS)), dim3(threads), 0, stream>>>(X + r * ldx, ldx, d, ldd, W, to,  \
+                                                                                ldsum, Q + r * ldq, ldq,          \
+                                                                                S + r * lds, lds, K, eps)
+    if (K < 8) QE_NORM(norm_mx8_kernel<1, true>);
+    else if (C == 1) QE_NORM(norm_mx8_kernel<1, false>);
+    else if (C == 2) QE_NORM(norm_mx8_kernel<2, false>);
+    else if (pieces <= 4 * NORM_THREADS) QE_NORM(norm_mx8_kernel<4, false>);
+    else QE_NORM(norm_mx8_wide_kernel);
+  }
 #undef QE_NORM
   return hipGetLastError();
 }

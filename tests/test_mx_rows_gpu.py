@@ -129,3 +129,27 @@ def test_rows_do_not_depend_on_others(native, K):
         for r in (0, 3, 5):
             q1, s1 = run(x[r: r + 1], d[r: r + 1])
             assert torch.equal(q[r], q1[0]) and torch.equal(s[r], s1[0])
+
+
+def test_more_rows_than_a_launch_has(native):
+    """Rows past 2^21 equal the same rows in a call of their own."""
+    n, K = (1 << 21) + 5, 32
+    g = C.gen(4)
+    tail = torch.randn(9, 2 * K, generator=g).to(BF).to(DEV)
+    x = torch.zeros(n, 2 * K, dtype=BF, device=DEV)
+    x[-9:] = tail
+    w, d = torch.randn(K, generator=g).to(BF).to(DEV), torch.randn(9, K, generator=g).to(BF).to(DEV)
+    big, small = (tuple(torch.full((m, k), 0x55, dtype=U8, device=DEV) for k in (K, 1)) for m in (n, 9))
+    native.swiglu_mx8(x, *big)
+    native.swiglu_mx8(tail, *small)
+    assert torch.equal(big[0][-9:], small[0]) and torch.equal(big[1][-9:], small[1]) and not big[0][:-9].any()
+    native.quant_mx8(x[:, :K], *big)
+    native.quant_mx8(tail[:, :K], *small)
+    assert torch.equal(big[0][-9:], small[0]) and torch.equal(big[1][-9:], small[1])
+    delta = torch.zeros(n, K, dtype=BF, device=DEV)
+    delta[-9:] = d
+    sums = torch.empty(n, K, dtype=BF, device=DEV), torch.empty(9, K, dtype=BF, device=DEV)
+    native.rmsnorm1p_mx8(x[:, :K], delta, w, *big, 1e-6, sums[0])
+    native.rmsnorm1p_mx8(tail[:, :K], d, w, *small, 1e-6, sums[1])
+    assert torch.equal(big[0][-9:], small[0]) and torch.equal(big[1][-9:], small[1])
+    assert torch.equal(sums[0][-9:], sums[1]) and not sums[0][:-9].any()
