@@ -147,13 +147,13 @@ static hipError_t gemm_rows(const Product& c, hipStream_t stream) {
 // Between the others decides what each would take, in us: what a call costs at once, the steps of 128 of K of the
 // workgroups that take turns on a CU (a little longer while every CU has one), a workgroup's start and end, and
 // outputs (MB; a split writes and reads fp32 as well). The constants are least squares over 120 calls from
-// 17 x 80 x 64 to 2048 x 34816 x 5120, on which the choice is 2 % behind the best kernel and split, 15 % at most. us,
+// 17 x 80 x 64 to 2048 x 34816 x 5120, on which the choice is 2 % behind the best kernel and split, 18 % at most. us,
 // tiles of 256 x 256 / 256 x 160 / 128 x 256 / 64 x 256 / 64 x 128 / 32 x 128 / 32 x 64:
 //   2048 x 34816 x 5120  281 / 295 / 326 / 425 / 491 / - / 1128
 //   2048 x 5120 x 6144   57 / 51 / 70 / 77 / 88 / - / 198
 //   1024 x 5120 x 5120   46 / 33 / 29 / 39 / 37 / - / 80
-//   64 x 34816 x 5120    44 / 37 / 35 / 32 / 39 / 41 / 46 (272 tiles of 64 x 128 on 256 CUs, 136 of 64 x 256)
-//   300 x 5120 x 6144    53 / 37 / 31 / 22 / 15 / 20 / 27
+//   64 x 34816 x 5120    45 / 37 / 35 / 32 / 39 / 41 / 46 (272 tiles of 64 x 128 on 256 CUs, 136 of 64 x 256)
+//   300 x 5120 x 6144    53 / 37 / 31 / 20 / 15 / 20 / 27
 //   687 x 1326 x 5056    - / - / - / - / 15.8 / 12.6 / -
 //   77 x 5001 x 6176     55 / 38 / 33 / 25 / 19 / 13.6 / 10.7
 // Splits: 128 x 5120 x 17408 on 64 x 128, 48 us in one part, 31 in 2, 34 in 4; 40 x 100 x 17408 on 32 x 64, 16 in one, 9
@@ -167,7 +167,7 @@ static const Cost costs[KINDS] = {{256, 256, 11.7, 0.91, 0.17, 0.0, 0.0, 0.22}, 
                                   {128, 256, 7.4, 0.53, 0.18, 0.0, 0.0, 0.26},
                                   {256, 160, 8.1, 0.63, 0.19, 0.0, 0.0, 0.28},
                                   {64, 128, 3.0, 0.25, 0.03, 1.2, 2.6, 0.32},  // in BlockKind's
-                                  {64, 256, 4.1, 0.37, 0.07, 2.0, 2.2, 0.35},
+                                  {64, 256, 4.0, 0.33, 0.12, 1.8, 2.2, 0.38},
                                   {32, 128, 2.7, 0.34, 0.03, 2.6, 2.6, 0.20},
                                   {32, 64, 2.4, 0.50, 0.00, 2.5, 2.6, 0.11}};
 

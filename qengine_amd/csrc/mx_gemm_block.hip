@@ -1,11 +1,13 @@
 // The product of 8-bit rows and a 4-bit weight for tens to hundreds of rows: small tiles, K shared by groups of waves
 // and, where there are few tiles, by workgroups.
 //
-// Bound by what a CU takes in: about 60 GB/s of lines that its L2 has to fetch, 90 of others, however many loads are
-// on the way (four or eight steps ahead, the weight through LDS or into registers, K begun elsewhere by every
-// workgroup: all the same), so that a tile's bytes a step decide: x 128 ROWS + w 64 COLS. 300 x 5120 x 6144 is 200
-// tiles of 64 x 128, 48 steps of 16 KB: 14.6 us, 1,290 TFLOP/s; 77 x 5001 x 6176 237 tiles of 32 x 64 whose four
-// parts of K run side by side, 13 steps of 32 KB: 10.7 us; 64 x 34816 x 5120 32 us.
+// Bound by a step's chain on a CU, no single part of it: a tile of 64 x 128 takes 0.2 us a step, of which 256 cycles
+// are products, 48 KB are read from LDS and 16 KB loaded. 320 x 5120 x 6144, 15.7 us: 12.6 without the products, 14.6
+// without the LDS reads, 12.1 without the loads, 11.4 with products and barriers alone; 13.9 and 14.7 with all of x
+// or of the weight from the L2. Deeper stages, one barrier for two steps, the weight straight into registers and
+// wider waves gave nothing or less. 300 x 5120 x 6144 14.7 us (200 tiles of 64 x 128); 77 x 5001 x 6176 10.6 us (237
+// of 32 x 64, four parts of K side by side, 13 steps); 64 x 34816 x 5120 31.7 us (136 of 64 x 256), bound by memory:
+// 22 us with the weight from the L2.
 #include <limits.h>
 
 #include <algorithm>
@@ -202,11 +204,15 @@ gemm_mx4_block_kernel(const BlockCall c) {
   int stage = 0;
   // A step, whose operands are in registers: the next step's are read behind the barrier (that stage has landed: only
   // the ST - 2 steps after it are out, and scales loaded since), the loads of the step ST ahead take the place of
-  // this one, which every wave has read ahead of the barrier, and this step's products run meanwhile.
+  // this one, which every wave has read ahead of the barrier. Reads and loads are issued between the step's products,
+  // or the matrix cores would wait until they all are (64 x 256 tiles, 300 x 5120 x 6144: 21.5 -> 19.5 us).
 #define QE_STEP(S, MORE)                                                                                      \
   {                                                                                                           \
     vmcnt_wait<(T::ST - 2) * T::LOADS + (MORE && S >= 1 && S <= T::ST - 2 ? SCALES : 0)>();                   \
     lds_barrier();                                                                                            \
+    __builtin_amdgcn_sched_barrier(0);                                                                        \
+    _Pragma("unroll") for (int i = 0; i < TX; ++i) _Pragma("unroll") for (int j = 0; j < TW; ++j) acc[i][j] = \
+        mfma32<S, 0>(a[S & 1][0][j], b[S & 1][0][i][0], b[S & 1][0][i][1], acc[i][j], sw[j][0], sx[i][S]);    \
     __builtin_amdgcn_sched_barrier(0);                                                                        \
     const int next = stage + 1 < T::ST ? stage + 1 : 0;                                                       \
     read(next, 1 - (S & 1));                                                                                  \
@@ -215,8 +221,6 @@ gemm_mx4_block_kernel(const BlockCall c) {
     __builtin_amdgcn_sched_barrier(0);                                                                        \
     fetch(s0 + S + T::ST, stage);                                                                             \
     __builtin_amdgcn_sched_barrier(0);                                                                        \
-    _Pragma("unroll") for (int i = 0; i < TX; ++i) _Pragma("unroll") for (int j = 0; j < TW; ++j) acc[i][j] = \
-        mfma32<S, 0>(a[S & 1][0][j], b[S & 1][0][i][0], b[S & 1][0][i][1], acc[i][j], sw[j][0], sx[i][S]);    \
     _Pragma("unroll") for (int i = 0; i < TX; ++i) _Pragma("unroll") for (int j = 0; j < TW; ++j) acc[i][j] = \
         mfma32<S, 2>(a[S & 1][1][j], b[S & 1][1][i][0], b[S & 1][1][i][1], acc[i][j], sw[j][1], sx[i][S]);    \
     _Pragma("unroll") for (int i = 0; i < TX; ++i) _Pragma("unroll") for (int j = 0; j < TW; ++j)             \
