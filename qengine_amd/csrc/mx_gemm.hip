@@ -182,9 +182,9 @@ static long tiles(const Cost& c, int n, int N) {
   return (long)((n + c.rows - 1) / c.rows) * ((N + c.cols - 1) / c.cols);
 }
 
-static double estimate(int kind, int splits, int n, int N, int K) {
+static double estimate(int kind, int splits, int n, int N, int K, long cus) {
   const Cost& c = costs[kind];
-  const double cus = compute_units(), turns = (double)tiles(c, n, N) * splits / cus, mb = 2e-6 * n * N;
+  const double turns = (double)tiles(c, n, N) * splits / cus, mb = 2e-6 * n * N;
   const int steps =
       kind < TILES ? std::max((K + 127) / 128, 2) : block_parts((BlockKind)(kind - TILES), K, splits).part;
   return c.call + std::ceil(turns) * steps * (c.step + c.full * std::min(turns, 1.)) + turns * c.group +
@@ -195,7 +195,7 @@ static size_t split_bytes(int n, int N, int splits) {
   return splits > 1 ? (size_t)splits * n * ((N + 15) / 16 * 16) * 4 : 0;
 }
 
-static Choice choose(int n, int N, int K, size_t ws_bytes) {
+static Choice choose(int n, int N, int K, size_t ws_bytes, long cus) {
   const Layout L(N, K);
   if (n <= 16 || (L.KS <= ROW_WAVES && (long)((n + 15) / 16) * L.RT * L.KS <= 2000)) return {ROWS, 1, 4.};
   Choice best = {ROWS, 1, 1e30};
@@ -204,7 +204,7 @@ static Choice choose(int n, int N, int K, size_t ws_bytes) {
       if (splits > 1 && (block_parts((BlockKind)(kind - TILES), K, splits).splits != splits ||
                          split_bytes(n, N, splits) > ws_bytes))
         continue;
-      const double us = estimate(kind, splits, n, N, K);
+      const double us = estimate(kind, splits, n, N, K, cus);
       if (us < best.us) best = {kind, splits, us};
     }
   return best;
@@ -219,17 +219,17 @@ struct Plan {
 };
 
 static Plan plan(int n, int N, int K, size_t ws_bytes) {
-  Plan best = {choose(n, N, K, ws_bytes), {}, N};
+  const long cus = compute_units();
+  Plan best = {choose(n, N, K, ws_bytes, cus), {}, N};
   if (best.first.kind == ROWS) return best;
   double least = 0.97 * best.first.us;
-  const long cus = compute_units();
   for (int kind = 0; kind < KINDS; ++kind) {
     const long all = tiles(costs[kind], n, N), xtiles = (n + costs[kind].rows - 1) / costs[kind].rows;
     const long cut = all / cus * cus / xtiles * costs[kind].cols;  // a multiple of 32
     if (cut <= 0 || cut >= N) continue;
-    const double us = estimate(kind, 1, n, (int)cut, K);
+    const double us = estimate(kind, 1, n, (int)cut, K, cus);
     if (us >= least) continue;
-    const Choice rest = choose(n, N - (int)cut, K, ws_bytes);
+    const Choice rest = choose(n, N - (int)cut, K, ws_bytes, cus);
     if (us + rest.us < least) least = us + rest.us, best = {{kind, 1, us}, rest, (int)cut};
   }
   return best;
