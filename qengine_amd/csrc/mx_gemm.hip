@@ -144,11 +144,13 @@ static hipError_t gemm_rows(const Product& c, hipStream_t stream) {
 // work is small and K short (us, it / the best of the others: 32 x 1000 x 1000 3.9 / 5.6, 102 x 171 x 2176 4.6 / 6.8;
 // past the rule 25 x 13906 x 128 4.8 / 5.4, 55 x 15157 x 352 8.2 / 6.9, 17 x 5120 x 6144 9.6 / 7.8).
 //
-// Between the others decides what each would take, in us: what a call costs at once, the steps of 128 of K of the
-// workgroups that take turns on a CU (a little longer while every CU has one), a workgroup's start and end, and
-// outputs (MB; a split writes and reads fp32 as well). The constants are least squares over 120 calls from
-// 17 x 80 x 64 to 2048 x 34816 x 5120, on which the choice is 2 % behind the best kernel and split, 18 % at most. us,
-// tiles of 256 x 256 / 256 x 160 / 128 x 256 / 64 x 256 / 64 x 128 / 32 x 128 / 32 x 64:
+// Between the others decides what each would take, in us: what a call costs at once; the steps of 128 of K of the
+// workgroups that take turns on a CU (a little longer while every CU has one), but no less than reading the weight at
+// 7 TB/s, longer by what the last turn leaves idle (32 x 34816 x 5120: 32.8 on 272 tiles of 32 x 128, 24.2 on 136 of
+// 64 x 256); a workgroup's start and end; and outputs (MB; a split writes and reads fp32 as well). The constants are
+// least squares over 120 calls from 17 x 80 x 64 to 2048 x 34816 x 5120, on which the choice is 2 % behind the best
+// kernel and split, 18 % at most. us, tiles of 256 x 256 / 256 x 160 / 128 x 256 / 64 x 256 / 64 x 128 / 32 x 128 /
+// 32 x 64:
 //   2048 x 34816 x 5120  281 / 295 / 326 / 425 / 491 / - / 1128
 //   2048 x 5120 x 6144   57 / 51 / 70 / 77 / 88 / - / 198
 //   1024 x 5120 x 5120   46 / 33 / 29 / 39 / 37 / - / 80
@@ -156,8 +158,8 @@ static hipError_t gemm_rows(const Product& c, hipStream_t stream) {
 //   300 x 5120 x 6144    53 / 37 / 31 / 20 / 15 / 20 / 27
 //   687 x 1326 x 5056    - / - / - / - / 15.8 / 12.6 / -
 //   77 x 5001 x 6176     55 / 38 / 33 / 25 / 19 / 13.6 / 10.7
-// Splits: 128 x 5120 x 17408 on 64 x 128, 48 us in one part, 31 in 2, 34 in 4; 40 x 100 x 17408 on 32 x 64, 16 in one, 9
-// in 4.
+// Splits: 128 x 5120 x 17408 on 64 x 128, 48 us in one part, 31 in 2, 34 in 4; 40 x 100 x 17408 on 32 x 64, 16 in
+// one, 9 in 4.
 struct Cost {
   int rows, cols;  // of a tile
   double call, step, full, group, split, out;
@@ -187,7 +189,9 @@ static double estimate(int kind, int splits, int n, int N, int K, long cus) {
   const double turns = (double)tiles(c, n, N) * splits / cus, mb = 2e-6 * n * N;
   const int steps =
       kind < TILES ? std::max((K + 127) / 128, 2) : block_parts((BlockKind)(kind - TILES), K, splits).part;
-  return c.call + std::ceil(turns) * steps * (c.step + c.full * std::min(turns, 1.)) + turns * c.group +
+  const double work = std::ceil(turns) * steps * (c.step + c.full * std::min(turns, 1.));
+  const double weight = N * (K * 17. / 32 / 7e6) * std::max(std::ceil(turns) / turns, 1.);
+  return c.call + std::max(work, weight) + turns * c.group +
          (splits > 1 ? c.split + c.out * mb * (2 * splits + 1) : c.out * mb);
 }
 

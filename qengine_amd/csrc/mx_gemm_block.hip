@@ -6,7 +6,7 @@
 // without the LDS reads, 12.1 without the loads, 11.4 with products and barriers alone; 13.9 and 14.7 with all of x
 // or of the weight from the L2. Deeper stages, one barrier for two steps, the weight straight into registers and
 // wider waves gave nothing or less. 300 x 5120 x 6144 14.7 us (200 tiles of 64 x 128); 77 x 5001 x 6176 10.6 us (237
-// of 32 x 64, four parts of K side by side, 13 steps); 64 x 34816 x 5120 31.7 us (136 of 64 x 256), bound by memory:
+// of 32 x 64, four parts of K side by side, 13 steps); 64 x 34816 x 5120 29.0 us (136 of 64 x 256), bound by memory:
 // 22 us with the weight from the L2.
 #include <limits.h>
 
@@ -37,7 +37,8 @@ struct BlockCall : Product {
   int part;  // 128-value tiles of a part of K
 };
 
-template <int WX, int WW, int WK, int TX, int TW, int STAGES, class T = Block<WX, WW, WK, TX, TW, STAGES>>
+template <int WX, int WW, int WK, int TX, int TW, int STAGES, bool ONCE,
+          class T = Block<WX, WW, WK, TX, TW, STAGES>>
 __global__ void __launch_bounds__(T::WAVES * WAVE, 2 * T::PER_CU)
 gemm_mx4_block_kernel(const BlockCall c) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[T::LDS];
@@ -88,7 +89,7 @@ gemm_mx4_block_kernel(const BlockCall c) {
     for (int i = 0; i < T::WL; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           wr, (__attribute__((address_space(3))) void*)(uintptr_t)(wl[i] + stage * T::STAGE), 16,
-          (int)(wo[i] + min(wkt[i] + s, KT - 1) * 1024), 0, 0, 0);
+          (int)(wo[i] + min(wkt[i] + s, KT - 1) * 1024), 0, 0, ONCE ? CPOL_NT : 0);
   };
 
   // Scales of four steps. Of x, 16 bytes of lane r's row, the last ones shifted down from the row's end: no byte past
@@ -306,8 +307,19 @@ static hipError_t run(const Product& p, int splits, hipStream_t stream) {
   const Parts k = parts(WK, p.K, splits);
   BlockCall c = {p, (int)xt, (int)wt, k.part};
   if (k.splits == 1) c.ws = nullptr;
-  gemm_mx4_block_kernel<WX, WW, WK, TX, TW, STAGES>
-      <<<dim3(xt * wt, k.splits), dim3(T::WAVES * WAVE), 0, stream>>>(c);
+  const dim3 grid(xt * wt, k.splits), block(T::WAVES * WAVE);
+  // A weight that is read once, and so large that no cache will hold it until the next call, passes the caches' favour:
+  // 64 x 34816 x 5120 (95 MB) 31.6 -> 29.0 us (smaller ones may still be there: 32 x 14336 x 5120, 41 MB, 9.6 us, 12.4
+  // past them; from memory 13.1 and 12.5).
+  if constexpr (T::ROWS == 64) {
+    if (xt == 1 && Layout(p.N, p.K).scales() >= 64u << 20) {
+      gemm_mx4_block_kernel<WX, WW, WK, TX, TW, STAGES, true><<<grid, block, 0, stream>>>(c);
+    } else {
+      gemm_mx4_block_kernel<WX, WW, WK, TX, TW, STAGES, false><<<grid, block, 0, stream>>>(c);
+    }
+  } else {
+    gemm_mx4_block_kernel<WX, WW, WK, TX, TW, STAGES, false><<<grid, block, 0, stream>>>(c);
+  }
   if (k.splits > 1)
     mx4_sum_kernel<<<dim3(p.n, (p.N + 1023) / 1024), dim3(256), 0, stream>>>(p.ws, p.out, p.ldo, p.n, p.N,
                                                                             (p.N + 15) / 16 * 16, k.splits);
