@@ -80,7 +80,7 @@ def test_every_remainder_of_k(native, n, N):
 
 # weight rows past the last whole turn of the CUs go to another kernel: odd ends, strides, a workspace for them alone
 @pytest.mark.parametrize("n,N,K", [(500, 33003, 2080), (64, 33001, 4096), (70, 16901, 8192), (1000, 17000, 2048),
-                                   (32, 33901, 5120)])
+                                   (32, 34815, 5120)])
 def test_wide_products(native, n, N, K):
     import qengine_amd as qa
     g = C.gen(N)
