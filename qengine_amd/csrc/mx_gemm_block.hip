@@ -6,8 +6,8 @@
 // without the LDS reads, 12.1 without the loads, 11.4 with products and barriers alone; 13.9 and 14.7 with all of x
 // or of the weight from the L2. Deeper stages, one barrier for two steps, the weight straight into registers and
 // wider waves gave nothing or less. 300 x 5120 x 6144 14.7 us (200 tiles of 64 x 128); 77 x 5001 x 6176 10.6 us (237
-// of 32 x 64, four parts of K side by side, 13 steps); 64 x 34816 x 5120 29.0 us (136 of 64 x 256), bound by memory:
-// 22 us with the weight from the L2.
+// of 32 x 64, four parts of K side by side, 13 steps); 64 x 34816 x 5120 28.8 us (256 of 64 x 128, and
+// 64 of 32 x 64 for the weight rows past them; 29.0 on 136 of 64 x 256), bound by memory.
 #include <limits.h>
 
 #include <algorithm>
@@ -308,9 +308,9 @@ static hipError_t run(const Product& p, int splits, hipStream_t stream) {
   BlockCall c = {p, (int)xt, (int)wt, k.part};
   if (k.splits == 1) c.ws = nullptr;
   const dim3 grid(xt * wt, k.splits), block(T::WAVES * WAVE);
-  // A weight that is read once, and so large that no cache will hold it until the next call, passes the caches' favour:
-  // 64 x 34816 x 5120 (95 MB) 31.6 -> 29.0 us (smaller ones may still be there: 32 x 14336 x 5120, 41 MB, 9.6 us, 12.4
-  // past them; from memory 13.1 and 12.5).
+  // A weight that is read once, and so large that no cache will hold it until the next call, passes the caches'
+  // favour: 64 x 34816 x 5120 (95 MB) on 64 x 256 31.6 -> 29.0 us (smaller ones may still be there: 32 x 14336 x
+  // 5120, 41 MB, 9.6 us, 12.4 past them; from memory 13.1 and 12.5).
   if constexpr (T::ROWS == 64) {
     if (xt == 1 && Layout(p.N, p.K).scales() >= 64u << 20) {
       gemm_mx4_block_kernel<WX, WW, WK, TX, TW, STAGES, true><<<grid, block, 0, stream>>>(c);
