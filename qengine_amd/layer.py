@@ -19,14 +19,13 @@ serves one sequence and has no counterpart.
 
 MX4Linear and MX4MLP are linear layers on 4-bit weights (microscaled E2M1 codes, where the reference's W4Linear has
 integers: python/qengine/engine.py:74-186) for decode rows and prompt chunks alike: MX4MLP is the second half of
-Engine._layer (engine.py:460-466), norm with the residual's addition, gate and up, SwiGLU, down, in four launches.
+Engine._layer (engine.py:460-466), norm with the residual's addition, gate and up, SwiGLU, down, in four calls.
 """
 from __future__ import annotations
 
 import torch
 
-from . import (_C, alloc_mx4, alloc_mx4_ws, alloc_mx8, alloc_pages_ws, alloc_partials, default_paged_splits,
-               default_splits)
+from . import (_C, alloc_mx4, alloc_mx8, alloc_pages_ws, alloc_partials, default_paged_splits, default_splits)
 
 HEAD_DIM = 256
 
