@@ -59,6 +59,7 @@ hipError_t qe_rmsnorm1p_mx8(const void* x, long ldx, const void* delta, long ldd
  * ws: qe_gemm_mx4_ws_size(n, N, K) bytes, 16-byte aligned, any contents, one per call in flight (NULL where that
  * is 0; with fewer bytes the call runs without it, in another order of sums). Graphs that share one must not be
  * replayed at the same time.
+ * qe_gemm_mx4_ws_size takes a weight's own width too: it is that of the rows, filled up to a multiple of 32.
  * Valid: n >= 1, N >= 1, K >= 32, ldx >= K and a multiple of 16, xq and wq 16-byte aligned, lds >= K / 32,
  * ldo >= N. */
 hipError_t qe_gemm_mx4(const void* wq, const void* xq, long ldx, const void* xs, long lds, void* out, long ldo,

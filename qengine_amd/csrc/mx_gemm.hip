@@ -246,7 +246,8 @@ using namespace qe;
 using namespace qe::mx;
 
 extern "C" size_t qe_gemm_mx4_ws_size(int n, int N, int K) {
-  if (!dims_ok(n, 1) || !dims_ok(N, K) || K % BLOCK) return 0;
+  if (!dims_ok(n, 1) || !dims_ok(N, K)) return 0;
+  K = (K + BLOCK - 1) / BLOCK * BLOCK;  // of the rows
   const Plan p = plan(n, N, K, SIZE_MAX);
   return p.cut < N ? split_bytes(n, N - p.cut, p.rest.splits) : split_bytes(n, N, p.first.splits);
 }

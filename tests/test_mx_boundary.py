@@ -149,3 +149,17 @@ def test_capi_rejects(capi, name):
     for kw in BAD[name]:
         assert fn(*{**C_CALLS[name], **kw}.values()) == INVALID, kw
     assert capi.load().qe_mx4_bytes(0, 5) == 0 and capi.load().qe_mx4_bytes(5, 1 << 21) == 0
+
+
+def test_workspace_of_any_width(native):
+    """A weight's own width asks for the workspace of the product, whose rows are filled up to a multiple of 32."""
+    import qengine_amd as qa
+    from qengine_amd import capi
+    assert native.mx4_ws_bytes(128, 5120, 17408) > 0  # K is split here
+    for n, N, K in ((128, 5120, 17401), (128, 5120, 17377), (100, 513, 17400), (40, 100, 9351), (300, 5120, 6113),
+                    (17, 1, 1), (1, 7, 33)):
+        want = native.mx4_ws_bytes(n, N, -(-K // 32) * 32)
+        assert native.mx4_ws_bytes(n, N, K) == want, (n, N, K)
+        assert capi.load().qe_gemm_mx4_ws_size(n, N, K) == want
+        assert qa.alloc_mx4_ws(n, N, K, device="cpu").numel() == want
+    assert native.mx4_ws_bytes(128, 5120, 2 ** 20) == native.mx4_ws_bytes(128, 5120, 2 ** 20 - 31)

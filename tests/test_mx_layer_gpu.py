@@ -76,3 +76,23 @@ def test_captured(mlp, n):
         layer(h2, b.to(DEV), ref)
         torch.cuda.synchronize()
         assert torch.equal(kept, ref) and torch.equal(after, h2), k
+
+
+@pytest.mark.parametrize("K", [17401, 17377])
+def test_linear_of_any_width(native, K):
+    """A layer whose width is no multiple of 32 has the workspace of its filled-up rows, and so the bits of a layer
+    that is filled up with zeros."""
+    from qengine_amd import alloc_mx8
+    from qengine_amd.layer import MX4Linear
+    n, N, Kp = 100, 513, -(-K // 32) * 32
+    g = C.gen(K)
+    w, x = C.randn(g, N, K, scale=K ** -0.5), C.randn(g, n, K).to(DEV)
+    layer, wide = (MX4Linear(t.to(DEV), rows=n) for t in (w, torch.nn.functional.pad(w, (0, Kp - K))))
+    assert layer.ws.numel() == wide.ws.numel() > 0
+    q, s = alloc_mx8(n, K)
+    native.quant_mx8(x, q, s)
+    out, same = torch.empty(n, N, dtype=BF, device=DEV), torch.empty(n, N, dtype=BF, device=DEV)
+    layer(q, s, out)
+    C.check_product(out, M.values8(q.cpu(), s.cpu()), M.values4(*M.quant4(w)), Kp)
+    wide(q, s, same)
+    assert torch.equal(out, same)
