@@ -3,6 +3,7 @@
 // device, never syncs or allocates, and raises RuntimeError for arguments outside its contract. The _check_*
 // functions run the same validation without the device requirement and without a launch.
 #include "bindings_util.hpp"
+#include "mx_form.hpp"
 #include "qe_mx.h"
 
 namespace {
@@ -175,6 +176,22 @@ void gemm_mx4(torch::Tensor wq, torch::Tensor xq, torch::Tensor xs, torch::Tenso
            "qe_gemm_mx4");
 }
 
+// A given kernel, for the tests of each at any size.
+void gemm_mx4_as(int64_t kernel, int64_t splits, torch::Tensor wq, torch::Tensor xq, torch::Tensor xs,
+                 torch::Tensor out, Opt ws) {
+  auto a = parse_gemm(wq, xq, xs, out, ws, false);
+  TORCH_CHECK(kernel >= -1 && kernel < 16 && splits >= 1 && splits <= 64 &&
+                  qe::mx::gemm_form_ok((int)kernel, (int)splits, a.o.n, (int)a.o.w, (int)a.x.q.w, a.ws_bytes),
+              "kernel ", kernel, " does not take this call in ", splits, " splits");
+  a = parse_gemm(wq, xq, xs, out, ws, true);
+  const c10::DeviceGuard guard(out.device());
+  raise_on(qe::mx::gemm_as((int)kernel, (int)splits,
+                           {wq.data_ptr(), xq.data_ptr(), a.x.q.ld, xs.data_ptr(), a.x.s.ld, out.data_ptr(), a.o.ld,
+                            a.o.n, (int)a.o.w, (int)a.x.q.w, a.ws, a.ws_bytes},
+                           stream_of(out)),
+           "gemm_mx4");
+}
+
 int64_t positive(int64_t v, int64_t most, const char* what) {
   TORCH_CHECK(v >= 1 && v <= most, what, " must be 1..", most, ", got ", v);
   return v;
@@ -222,4 +239,12 @@ void bind_mx(py::module_& m) {
     const auto a = parse_gemm(wq, xq, xs, out, ws, false);
     return std::vector<int64_t>{a.o.n, a.o.w, a.x.q.w, a.x.q.ld, a.x.s.ld, a.o.ld};
   });
+  // how gemm_mx4 runs a call (host only): (kernel, splits, weight rows of that, kernel and splits of the others)
+  m.def("_gemm_mx4_form", [](int64_t n, int64_t N, int64_t K, int64_t ws_bytes) {
+    TORCH_CHECK(ws_bytes >= 0 && K % 32 == 0, "K is a multiple of 32, a workspace has no negative size");
+    const auto f = qe::mx::gemm_form((int)positive(n, QE_MX_MAX_ROWS, "n"), (int)positive(N, QE_MX_MAX_ROWS, "N"),
+                                     (int)positive(K, QE_MX_MAX_WIDTH, "K"), (size_t)ws_bytes);
+    return std::make_tuple(f.kernel, f.splits, f.cut, f.rest_kernel, f.rest_splits);
+  });
+  m.def("_gemm_mx4_as", &gemm_mx4_as);
 }

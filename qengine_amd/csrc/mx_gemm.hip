@@ -7,6 +7,7 @@
 #include <cmath>
 
 #include "mx_common.hpp"
+#include "mx_form.hpp"
 #include "mx_gemm.hpp"
 
 namespace qe {
@@ -258,21 +259,29 @@ static hipError_t run(const Choice& c, const Product& p, hipStream_t stream) {
   return gemm_blocks((BlockKind)(c.kind - TILES), c.splits, p, stream);
 }
 
+static bool product_ok(const GemmArgs& a) {
+  return a.wq && a.xq && a.xs && a.out && dims_ok(a.n, a.K) && dims_ok(a.N, a.K) && a.K % BLOCK == 0 &&
+         ld_ok(a.ldx, a.K) && a.ldx % 16 == 0 && ld_ok(a.lds, a.K / BLOCK) && ld_ok(a.ldo, a.N) &&
+         aligned(a.wq, 16) && aligned(a.xq, 16) && aligned(a.out, 2) && aligned(a.ws, 16);
+}
+
+static Product product(const GemmArgs& a) {
+  return {static_cast<const uint8_t*>(a.wq),
+          static_cast<const uint8_t*>(a.wq) + Layout(a.N, a.K).scales(),
+          static_cast<const uint8_t*>(a.xq),
+          static_cast<const uint8_t*>(a.xs),
+          static_cast<__bf16*>(a.out),
+          static_cast<float*>(a.ws),
+          a.ldx, a.lds, a.ldo, a.n, a.N, a.K};
+}
+
 extern "C" hipError_t qe_gemm_mx4(const void* wq, const void* xq, long ldx, const void* xs, long lds, void* out,
                                   long ldo, int n, int N, int K, void* ws, size_t ws_bytes, hipStream_t stream) {
-  if (!wq || !xq || !xs || !out || !dims_ok(n, K) || !dims_ok(N, K) || K % BLOCK || !ld_ok(ldx, K) || ldx % 16 ||
-      !ld_ok(lds, K / BLOCK) || !ld_ok(ldo, N) || !aligned(wq, 16) || !aligned(xq, 16) || !aligned(out, 2) ||
-      !aligned(ws, 16))
-    return hipErrorInvalidValue;
+  const GemmArgs a = {wq, xq, ldx, xs, lds, out, ldo, n, N, K, ws, ws ? ws_bytes : 0};
+  if (!product_ok(a)) return hipErrorInvalidValue;
   const Layout L(N, K);
-  Product p = {static_cast<const uint8_t*>(wq),
-               static_cast<const uint8_t*>(wq) + L.scales(),
-               static_cast<const uint8_t*>(xq),
-               static_cast<const uint8_t*>(xs),
-               static_cast<__bf16*>(out),
-               static_cast<float*>(ws),
-               ldx, lds, ldo, n, N, K};
-  const Plan how = plan(n, N, K, ws ? ws_bytes : 0);
+  Product p = product(a);
+  const Plan how = plan(n, N, K, a.ws_bytes);
   p.N = how.cut;
   const hipError_t e = run(how.first, p, stream);
   if (e != hipSuccess || how.cut == N) return e;
@@ -282,3 +291,28 @@ extern "C" hipError_t qe_gemm_mx4(const void* wq, const void* xq, long ldx, cons
   p.N = N - how.cut;
   return run(how.rest, p, stream);
 }
+
+// ------------------------------------------------------------------------------ for the tests
+namespace qe {
+namespace mx {
+
+Form gemm_form(int n, int N, int K, size_t ws_bytes) {
+  const Plan p = plan(n, N, K, ws_bytes);
+  return {p.first.kind, p.first.splits, p.cut, p.rest.kind, p.rest.splits};
+}
+
+bool gemm_form_ok(int kernel, int splits, int n, int N, int K, size_t ws_bytes) {
+  if (kernel < ROWS || kernel >= KINDS) return false;
+  if (kernel < TILES) return splits == 1 && (kernel != ROWS || (n + 15) / 16 <= 65535);  // a grid's second axis
+  return splits >= 1 && block_parts((BlockKind)(kernel - TILES), K, splits).splits == splits &&
+         split_bytes(n, N, splits) <= ws_bytes;
+}
+
+hipError_t gemm_as(int kernel, int splits, const GemmArgs& a, hipStream_t stream) {
+  if (!product_ok(a) || !gemm_form_ok(kernel, splits, a.n, a.N, a.K, a.ws ? a.ws_bytes : 0))
+    return hipErrorInvalidValue;
+  return run({kernel, splits, 0.}, product(a), stream);
+}
+
+}  // namespace mx
+}  // namespace qe

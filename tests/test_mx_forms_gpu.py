@@ -1,0 +1,273 @@
+"""Each kernel of the product on 4-bit weights by itself, whatever the choice between them would take, on the GPU against
+the 64-bit product: every tail of K, ragged rows and weight rows, workgroups that take several tiles, splits, NaN,
+repeated and captured calls; and the streaming kernel on long sums, for one to 16 rows."""
+import pytest
+import torch
+
+import mx_cases as C
+from oracle import mx_oracle as M
+
+pytestmark = pytest.mark.gpu
+BF, F64, U8, DEV = C.BF, C.F64, C.U8, C.DEV
+
+ROWS = -1
+TILES = {0: (256, 256), 1: (128, 256), 2: (256, 160), 3: (64, 128), 4: (64, 256), 5: (32, 128), 6: (32, 64)}
+
+
+def rows8(g, n, K):
+    """Codes of every value but NaN, under scales far apart."""
+    q = torch.randint(0, 127, (n, K), generator=g) + 128 * torch.randint(0, 2, (n, K), generator=g)
+    return q.to(U8), torch.randint(113, 140, (n, K // 32), generator=g).to(U8)
+
+
+def weights(native, g, N, K):
+    """A weight's 4-bit form, and its values as the dequantiser reads them (bit for bit elsewhere)."""
+    import qengine_amd as qa
+    w = (torch.randn(N, K, generator=g) * torch.exp2(torch.randint(-4, 5, (N, 1), generator=g).float())).to(BF).to(DEV)
+    wq = qa.alloc_mx4(N, K)
+    native.mx4_quant(w, wq)
+    native.mx4_dequant(wq, w)
+    return wq, w.to(F64)
+
+
+def placed(q, s, N, aligned):
+    """Rows as they are, or inside wider buffers whose scale rows start at odd bytes; an output surrounded by sevens."""
+    n, K = q.shape
+    if aligned:
+        out = torch.full((n + 1, (N + 63) // 64 * 64 + 64), 7.0, dtype=BF, device=DEV)
+        return q.to(DEV), s.to(DEV), out, out[:n, :N]
+    qd = torch.full((n, K + 48), 0x7F, dtype=U8, device=DEV)[:, 16: 16 + K]
+    sd = torch.full((n, K // 32 + 3), 0xFF, dtype=U8, device=DEV)[:, 1: 1 + K // 32]
+    big = torch.full((n + 1, N + 5), 7.0, dtype=BF, device=DEV)
+    return qd.copy_(q), sd.copy_(s), big, big[:n, 3: 3 + N]
+
+
+def check(native, kernel, splits, q, s, wq, wv, ws, aligned):
+    n, K, N = *q.shape, len(wv)
+    qd, sd, big, out = placed(q, s, N, aligned)
+    out.fill_(float("nan"))
+    if ws is not None:
+        ws.fill_(0xFF)
+    native._gemm_mx4_as(kernel, splits, wq, qd, sd, out, ws)
+    C.check_product(out, M.values8(q, s), wv, K)
+    first = out.clone()
+    native._gemm_mx4_as(kernel, splits, wq, qd, sd, out, ws)  # the same bits again
+    assert torch.equal(first, out)
+    left = 0 if aligned else 3
+    assert (big[n] == 7).all() and (big[:, :left] == 7).all() and (big[:, left + N:] == 7).all()
+    return first
+
+
+# every number of blocks to a tile of K, of tiles to a group of four, fewer and more than 16 blocks
+BLOCKS = [*range(1, 22), 24, 25, 27, 28, 29, 31, 32, 33, 36, 37, 40, 44, 48, 49, 52, 56, 60, 61, 64, 67, 83]
+
+
+@pytest.mark.parametrize("kernel", [ROWS, *TILES])
+def test_every_tail_of_k(native, kernel):
+    rows, cols = TILES.get(kernel, (16, 64))
+    n, N = rows + rows // 2 + 3, 2 * cols + cols // 2 + 5
+    for b in BLOCKS:
+        g = C.gen(b + 1000 * kernel)
+        q, s = rows8(g, n, 32 * b)
+        wq, wv = weights(native, g, N, 32 * b)
+        check(native, kernel, 1, q, s, wq, wv, None, b % 2 == 0)
+
+
+@pytest.mark.parametrize("kernel", [ROWS, *TILES])
+def test_ragged_rows_and_weight_rows(native, kernel):
+    """From a single output to one past whole tiles; outputs on whole lines and not."""
+    rows, cols = TILES.get(kernel, (16, 64))
+    for n, N, K in ((1, 1, 32), (2, 8, 160), (rows, cols, 544), (rows - 1, cols + 1, 544), (rows + 1, cols - 1, 672),
+                    (17, 2 * cols + 16, 1056), (rows + 33, 31, 416), (5, cols + 9, 96), (3 * rows, 24, 608)):
+        g = C.gen(n + N + kernel)
+        q, s = rows8(g, n, K)
+        wq, wv = weights(native, g, N, K)
+        a, b = (check(native, kernel, 1, q, s, wq, wv, None, aligned) for aligned in (True, False))
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("K", [32, 128, 160, 352, 416, 544, 672, 800, 1024])
+@pytest.mark.parametrize("kernel", [0, 1, 2])
+def test_workgroups_that_take_several_tiles(native, kernel, K):
+    """More tiles than the card has CUs: the loads of a tile's first steps pass in the one before it."""
+    rows, cols = TILES[kernel]
+    n, N = rows + 7, 132 * cols + 3  # 266 tiles
+    g = C.gen(K + kernel)
+    q, s = rows8(g, n, K)
+    wq, wv = weights(native, g, N, K)
+    check(native, kernel, 1, q, s, wq, wv, None, K % 64 == 0)
+
+
+@pytest.mark.parametrize("kernel", [3, 4, 5, 6])
+def test_splits(native, kernel):
+    rows, cols = TILES[kernel]
+    n, N = rows + 5, cols + 13
+    ran = set()
+    for b in (8, 12, 15, 20, 29, 33, 36, 37, 44, 61, 64, 68, 83, 96, 110, 128, 131, 134, 193, 261, 264, 266, 330, 544):
+        K, g = 32 * b, C.gen(b)
+        q, s = rows8(g, n, K)
+        wq, wv = weights(native, g, N, K)
+        for splits in (2, 3, 4, 8):
+            need = splits * n * (-(-N // 16) * 16) * 4
+            ws = torch.empty(need + 256, dtype=U8, device=DEV)
+            try:
+                native._gemm_mx4_as(kernel, splits, wq, q.to(DEV), s.to(DEV),
+                                    torch.empty(n, N, dtype=BF, device=DEV), ws[:need])
+            except RuntimeError as e:  # K has no so many parts
+                assert "does not take" in str(e)
+                continue
+            ran.add(splits)
+            check(native, kernel, splits, q, s, wq, wv, ws[:need], b % 2 == 0)
+            ws.fill_(0x55)
+            native._gemm_mx4_as(kernel, splits, wq, q.to(DEV), s.to(DEV),
+                                torch.empty(n, N, dtype=BF, device=DEV), ws[:need])
+            assert (ws[need:] == 0x55).all()
+    assert ran == {2, 3, 4, 8}
+
+
+@pytest.mark.parametrize("kernel", [3, 4])
+def test_weights_past_the_caches(native, kernel):
+    """One tile of rows on 64 MB of codes or more: the loads that pass the caches' favour."""
+    n, N, K = 33, 33001, 4128
+    g = C.gen(kernel)
+    q, s = rows8(g, n, K)
+    wq, wv = weights(native, g, N, K)
+    check(native, kernel, 1, q, s, wq, wv, None, kernel == 3)
+
+
+@pytest.mark.parametrize("K", [96, 416, 480, 1056, 1184])
+@pytest.mark.parametrize("kernel", [ROWS, *TILES])
+def test_nan_stays_in_its_row_and_column(native, kernel, K):
+    """A NaN scale of a row's last block, a NaN code, a NaN block of a weight row; the next rows in the same tile and
+    the padding beside them hold ordinary values."""
+    rows, cols = TILES.get(kernel, (16, 64))
+    n, N = rows + 9, cols + 21
+    g = C.gen(K + kernel)
+    q, s = rows8(g, n, K)
+    w = torch.randn(N, K, generator=g).to(BF)
+    r, j = n // 2, N - 3
+    s[r, K // 32 - 1] = 255
+    q[0, 3] = 0x7F
+    w[j, K - 1] = float("inf")
+    w[1, 7] = float("nan")
+    wq, wv = C.weight(native, w)
+    splits = 1
+    out = torch.empty(n, N, dtype=BF, device=DEV)
+    native._gemm_mx4_as(kernel, splits, wq, q.to(DEV), s.to(DEV), out, None)
+    want = torch.zeros(n, N, dtype=torch.bool)
+    want[r], want[0], want[:, j], want[:, 1] = True, True, True, True
+    assert torch.equal(torch.isnan(out.cpu()), want)
+    rows_, cols_ = ~want[:, 2], ~want[1]
+    C.check_product(out.cpu()[rows_][:, cols_], M.values8(q, s)[rows_], wv[cols_], K)
+
+
+@pytest.mark.parametrize("kernel,splits", [(ROWS, 1), (0, 1), (1, 1), (2, 1), (3, 1), (3, 4), (4, 2), (5, 2), (6, 1),
+                                           (6, 2)])
+def test_captured(native, kernel, splits):
+    """Replays on changed rows, with eager calls of the same kernel between them."""
+    rows, cols = TILES.get(kernel, (16, 64))
+    n, N, K = rows + 11, 3 * cols + 7, 1696
+    g = C.gen(kernel)
+    wq, wv = weights(native, g, N, K)
+    q, s = (t.to(DEV) for t in rows8(g, n, K))
+    ws, ws2 = (torch.empty(splits * n * (N + 16) * 4 // 16 * 16, dtype=U8, device=DEV) for _ in range(2))
+    out, ref = (torch.empty(n, N, dtype=BF, device=DEV) for _ in range(2))
+    native._gemm_mx4_as(kernel, splits, wq, q, s, out, ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        native._gemm_mx4_as(kernel, splits, wq, q, s, out, ws)
+    for k in range(4):
+        a, b = rows8(g, n, K)
+        q.copy_(a)
+        s.copy_(b)
+        out.fill_(float("nan"))
+        graph.replay()
+        native._gemm_mx4_as(kernel, splits, wq, q, s, ref, ws2)
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref), k
+        C.check_product(out, M.values8(a, b), wv, K)
+
+
+# one, two and four tiles a workgroup; K of two to three groups of 512 a wave, the last wave with one or none to share
+@pytest.mark.parametrize("K", [8224, 8704, 17408])
+@pytest.mark.parametrize("N", [264, 5125, 12307])
+def test_decode_rows_on_long_sums(native, N, K):
+    """2 to 16 rows on the MLP's second matrix: right, and with the bits of calls on each row alone."""
+    g = C.gen(N + K)
+    q, s = rows8(g, 16, K)
+    wq, wv = weights(native, g, N, K)
+    xv = M.values8(q, s)
+    q, s = q.to(DEV), s.to(DEV)
+    alone = torch.empty(16, N, dtype=BF, device=DEV)
+    for r in range(16):
+        native.gemm_mx4(wq, q[r: r + 1], s[r: r + 1], alone[r: r + 1])
+    C.check_product(alone, xv, wv, K)
+    for n in range(2, 17):
+        out = torch.full((n, N), float("nan"), dtype=BF, device=DEV)
+        native.gemm_mx4(wq, q[:n], s[:n], out)
+        assert torch.equal(out, alone[:n]), n
+
+
+def test_decode_rows_from_two_to_four_tiles(native):
+    """The gate and up weight: eight rows and nine are run by different forms of the kernel, with the same bits."""
+    N, K = 12305, 5120
+    g = C.gen(2)
+    q, s = rows8(g, 16, K)
+    wq, wv = weights(native, g, N, K)
+    xv = M.values8(q, s)
+    q, s = q.to(DEV), s.to(DEV)
+    alone = torch.empty(16, N, dtype=BF, device=DEV)
+    for r in range(16):
+        native.gemm_mx4(wq, q[r: r + 1], s[r: r + 1], alone[r: r + 1])
+    C.check_product(alone, xv, wv, K)
+    for n in (2, 5, 7, 8, 9, 12, 15, 16):
+        out = torch.full((n, N), float("nan"), dtype=BF, device=DEV)
+        native.gemm_mx4(wq, q[:n], s[:n], out)
+        assert torch.equal(out, alone[:n]), n
+
+
+@pytest.mark.parametrize("n,N,K", [(1500, 5001, 6176), (600, 8003, 4128), (1000, 17003, 2080)])
+def test_prompts_on_odd_sizes(native, n, N, K):
+    """Products as they are called, which tiles of 128 x 256 and 256 x 160 take."""
+    import qengine_amd as qa
+    g = C.gen(n)
+    q, s = rows8(g, n, K)
+    wq, wv = weights(native, g, N, K)
+    for aligned in (True, False):
+        qd, sd, big, out = placed(q, s, N, aligned)
+        native.gemm_mx4(wq, qd, sd, out, qa.alloc_mx4_ws(n, N, K))
+        C.check_product(out, M.values8(q, s), wv, K)
+        assert (big[n] == 7).all()
+
+
+def test_values_of_weights_past_32_bits(native):
+    """A weight of 4.4 GB of codes whose ordinary rows lie at its start, on both sides of 2^32 bytes of the source and
+    of the codes, around row 262144 (where a cut of 256-row tiles would fall) and at its end."""
+    import qengine_amd as qa
+    N, K = 270016, 32768
+    w = torch.zeros(N, K, dtype=BF, device=DEV)
+    g = C.gen(8)
+    at = torch.cat([torch.arange(a, a + 24) for a in (0, 65520, 131060, 262132, N - 24)])
+    some = (torch.randn(len(at), K, generator=g) * K ** -0.5).to(BF).to(DEV)
+    w[at] = some
+    wq = qa.alloc_mx4(N, K)
+    native.mx4_quant(w, wq)
+    del w
+    small = qa.alloc_mx4(len(at), K)
+    native.mx4_quant(some, small)
+    native.mx4_dequant(small, some)
+    others = torch.ones(N, dtype=torch.bool, device=DEV)
+    others[at] = False
+    for n, kernels in ((3, [ROWS]), (300, [ROWS, *TILES])):
+        q, s = rows8(g, n, K)
+        xv = M.values8(q, s)
+        q, s, out = q.to(DEV), s.to(DEV), torch.empty(n, N, dtype=BF, device=DEV)
+        for kernel in (None, *kernels):
+            out.fill_(float("nan"))
+            if kernel is None:
+                native.gemm_mx4(wq, q, s, out)
+            else:
+                native._gemm_mx4_as(kernel, 1, wq, q, s, out, None)
+            C.check_product(out[:, at], xv, some.to(F64), K)
+            assert not out[:, others].any(), (n, kernel)
