@@ -45,7 +45,7 @@ struct Place {
 
 __global__ void __launch_bounds__(256)
 mx4_quant_kernel(const __bf16* __restrict__ w, long ldw, uint8_t* __restrict__ wq, int N, int K) {
-  __shared__ uint8_t scales[WAVE][4];
+  __shared__ uint32_t scales[WAVE];  // a lane's four, by bytes
   const Layout L(N, K);
   const Place p(L);
   const int kt = p.J * 4 + p.t, k = kt * 128 + p.g * BLOCK + 8 * p.q;
@@ -81,11 +81,11 @@ mx4_quant_kernel(const __bf16* __restrict__ w, long ldw, uint8_t* __restrict__ w
   }
   if (kt < L.KT)
     reinterpret_cast<u32x4_t*>(wq + ((size_t)p.rt * L.KT + kt) * 1024)[p.code_lane()] = quad_transpose(codes, p.q);
-  scales[p.code_lane()][p.t] = kt < L.KT ? (uint8_t)mine : 0;
+  reinterpret_cast<uint8_t*>(scales + p.code_lane())[p.t] = kt < L.KT ? (uint8_t)mine : 0;
   __syncthreads();
   if (p.t == 0)
     reinterpret_cast<uint32_t*>(wq + L.scales() + ((size_t)p.rt * L.KS + p.J) * 256)[threadIdx.x] =
-        reinterpret_cast<const uint32_t*>(scales)[threadIdx.x];
+        scales[threadIdx.x];
 }
 
 __global__ void __launch_bounds__(256)
