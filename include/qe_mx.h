@@ -40,7 +40,8 @@ hipError_t qe_mx4_dequant(const void* wq, void* out, long ldo, int N, int K, hip
  * ceil(K / 32) wide. q 16-byte aligned, ldq a multiple of 16. Row r is computed exactly as in a 1-row call.
  *
  * qe_quant_mx8: of x [n][ldx] bf16.
- * qe_swiglu_mx8: of silu(g) * u in fp32, gu [n][ldg] = [g (K) | u (K)] bf16.
+ * qe_swiglu_mx8: of silu(g) * u in fp32, gu [n][ldg] = [g (K) | u (K)] bf16: off by at most (|g| + 8) 2^-23 of the
+ * value (and 2^-142), also where e^g leaves fp32's range.
  * qe_rmsnorm1p_mx8: of x * rsqrt(mean(x^2) + eps) * (1 + w) in fp32, w [K] bf16. With delta [n][ldd], x is
  * bf16(x + delta) and is written to sum [n][ldsum] (sum may be x itself, or delta); without, sum is NULL. */
 hipError_t qe_quant_mx8(const void* x, long ldx, void* q, long ldq, void* s, long lds, int n, int K,

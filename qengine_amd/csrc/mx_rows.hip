@@ -60,10 +60,18 @@ __device__ __forceinline__ void store8(const float (&v)[8], uint8_t* q, uint8_t*
   if ((c & 3) == 0) s[c >> 2] = (uint8_t)code;
 }
 
-// silu(g) * u: exp and the reciprocal are the instructions' (1 ulp each), about 2^-22 relative in all, far below
-// the code's 2^-4.
+// silu(g) * u, g >= FAR. exp and the reciprocal are the instructions' (1 ulp each, 2^-23); the exponential's argument is
+// off by 2^-24 (its rounding) and 2^-26 (the constant's) of itself. In all (0.61 |g| + 4) 2^-23 of the value, 2^-17 at
+// the most, far below the code's 2^-4.
+constexpr float FAR = -64.f;
 __device__ __forceinline__ float swiglu(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g)) * u;
+}
+// The same below FAR, where 1 + e^-g is e^-g in fp32 and leaves its range from g = -88 on, while g e^g u need not: e^g as a
+// fraction in [1/2, 1) and an exponent that u takes first. Nothing below -300 has a code.
+__device__ __forceinline__ float swiglu_far(float g, float u) {
+  const float x = fmaxf(1.44269504f * g, -300.f), e = floorf(x) + 1.f;
+  return g * ldexpf(__builtin_amdgcn_exp2f(x - e) * u, (int)e);
 }
 
 // ------------------------------------------------------------------------------ SwiGLU, plain rows
@@ -79,8 +87,17 @@ act_mx8_kernel(const __bf16* __restrict__ x, long ldx, uint8_t* __restrict__ q, 
   if constexpr (GLU) {
     float u[8];
     load8<TINY>(xr + K, c, K, u);
+    float g[8], least = v[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = swiglu(v[i], u[i]);
+    for (int i = 0; i < 8; ++i) {
+      g[i] = v[i];
+      least = fminf(least, g[i]);
+      v[i] = swiglu(g[i], u[i]);
+    }
+    if (least < FAR) {  // hardly ever
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = g[i] < FAR ? swiglu_far(g[i], u[i]) : v[i];
+    }
   }
   store8(v, q + r * ldq, s + r * lds, c, c < (K + BLOCK - 1) / BLOCK * 4);
 }

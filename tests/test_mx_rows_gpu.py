@@ -153,3 +153,44 @@ def test_more_rows_than_a_launch_has(native):
     native.rmsnorm1p_mx8(tail[:, :K], d, w, *small, 1e-6, sums[1])
     assert torch.equal(big[0][-9:], small[0]) and torch.equal(big[1][-9:], small[1])
     assert torch.equal(sums[0][-9:], sums[1]) and not sums[0][:-9].any()
+
+
+@pytest.mark.parametrize("K", [4096, 4091])
+def test_swiglu_far_gates(native, K):
+    """Gates down to -180, where e^g leaves fp32's range and silu(g) * u need not, and the largest ones; the block's
+    values are all of one gate's size, or beside ordinary ones."""
+    g = C.gen(K)
+    gate = torch.linspace(-180.0, -50.0, K).repeat(8, 1)  # a block's gates are within 1.1 of each other
+    up = torch.tensor([1.0, -3e2, 1e4, -1e10, 1e20, -1e30, 1.5e38, 1e-3])[:, None]
+    up = up * (1 + 0.1 * torch.rand(8, K, generator=g))
+    gate += 0.25 * torch.arange(8)[:, None]
+    gate[::2, 7::640], gate[1::2, 7::640] = 2.0, -3.3e38
+    gu = torch.cat([gate, up], 1).to(BF)
+    _, _, q, s = C.out8(8, K)
+    native.swiglu_mx8(gu.to(DEV), q, s)
+    q, s = q.cpu(), s.cpu()
+    y = M.blocks(M.swiglu(gu))
+    # relative: as in test_swiglu; past fp32's normal range u e^g is off by half of 2^-149, |g| times that in the end
+    d, a = (180 + 8) * 2.0 ** -23, 256 * 2.0 ** -150
+    lo, hi = M.scale_codes((y.abs() * (1 - d) - a).clamp(min=0), M.GRID8), M.scale_codes(y.abs() * (1 + d) + a, M.GRID8)
+    got = s.long()
+    assert ((got >= lo) & (got <= hi)).all()
+    scale = M.scale_values(got)[..., None]
+    v = y / scale
+    have = M.values8(q, torch.full_like(s, 127)).view(v.shape)
+    off = (have - v).abs() - (M.GRID8[M.nearest(v, M.GRID8)] - v.abs()).abs()
+    assert (off <= 2 * (d * v.abs() + a / scale)).all(), float((off / (d * v.abs() + a / scale)).max())
+    assert torch.equal(torch.signbit(have), torch.signbit(v))
+
+
+def test_swiglu_largest_gates(native):
+    """Infinities, and gates as large as bf16 has: -inf makes its block NaN, as silu(-inf) = -inf * 0 is; the largest
+    negative one is 0, with the sign of -u."""
+    g = torch.full((3, 64), -100.0)
+    g[0, 3], g[1, 40], g[2, 9] = -float("inf"), -3.38e38, float("inf")
+    u = torch.full((3, 64), 2.0)
+    u[1, 40] = -3e38
+    _, _, q, s = C.out8(3, 64)
+    native.swiglu_mx8(torch.cat([g, u], 1).to(BF).to(DEV), q, s)
+    assert (s.cpu() == 255).tolist() == [[True, False], [False, False], [True, False]]
+    assert int(q[1, 40]) == 0 and (q[1, :32] == 0x81).all()  # -200 e^-100 is 0.65 of the least code
