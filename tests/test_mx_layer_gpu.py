@@ -96,3 +96,42 @@ def test_linear_of_any_width(native, K):
     C.check_product(out, M.values8(q.cpu(), s.cpu()), M.values4(*M.quant4(w)), Kp)
     wide(q, s, same)
     assert torch.equal(out, same)
+
+
+def test_layers_that_share_their_scratch(native):
+    """Two layers one after another on one scratch: the bits of layers that own theirs, eagerly and as one graph."""
+    from qengine_amd.layer import MX4MLP
+    g = C.gen(21)
+    n, hidden, inner = 70, 512, 17408  # the second product has a workspace
+    made = []
+    for _ in range(2):
+        made.append([t.to(DEV) for t in (C.randn(g, hidden, scale=0.1), C.randn(g, 2 * inner, hidden, scale=hidden ** -0.5),
+                                         C.randn(g, hidden, inner, scale=inner ** -0.5))])
+    own = [MX4MLP(*w, EPS, rows=n) for w in made]
+    first = MX4MLP(*made[0], EPS, rows=n)
+    second = MX4MLP(*made[1], EPS, rows=n, share=first)
+    assert first.down.ws.numel() > 0
+    for a, b in ((first.x, second.x), (first.act, second.act), ((first.gu, first.down.ws), (second.gu, second.down.ws))):
+        assert [t.data_ptr() for t in a] == [t.data_ptr() for t in b]
+    h, d = C.randn(g, n, hidden, scale=3.0).to(DEV), C.randn(g, n, hidden).to(DEV)
+
+    def run(layers, h, d, out):
+        for layer in layers:
+            layer(h, d, out)
+            d = out
+    want, want_h = torch.empty_like(h), h.clone()
+    run(own, want_h, d, want)
+    got, got_h = torch.empty_like(h), h.clone()
+    run((first, second), got_h, d, got)
+    assert torch.equal(got, want) and torch.equal(got_h, want_h)
+    static, out = h.clone(), torch.empty_like(h)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run((first, second), static, d, out)
+    for _ in range(3):
+        static.copy_(h)
+        graph.replay()
+        run((first, second), h.clone(), d, got)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(static, want_h) and torch.equal(got, want)
