@@ -118,8 +118,16 @@ gemm_mx4_rows_kernel(const Product c, int per) {
 }
 
 // Tiles of a workgroup: two, so that a row of x is read half as often, while that leaves as many workgroups as 5/8 of
-// the CUs; four where x has more rows than the loads of two hide (us of 1 / 2 / 4: 1 x 5120 x 17408 13.5 / 12.3 /
-// 20.7, 3 x 1393 x 1472 4.0 / 4.1 / 4.9, 16 x 34816 x 5120 31.8 / 25.2 / 24.9, 16 x 14336 x 5120 - / 11.2 / 10.0).
+// the CUs; four where x has more rows than the loads of two hide. us of 1 / 2 / 4 on N weight rows:
+//   K = 5120   N 4096            5120              8192              12288             14336
+//    1 row     4.5 / 5.1 / 6.7   5.8 / 5.4 / 6.9   6.8 / 6.1 / 7.5   10.3 / 9.6 / 8.9  11.7 / 10.1 / 9.4
+//    16 rows   6.2 / 6.8 / 8.5   9.2 / 7.0 / 8.6   9.6 / 7.6 / 9.1   12.7 / 12 / 9.8   18.7 / 12.8 / 10.4
+//   K = 17408
+//    5 rows    11.7 / 13.1 / 21  16.3 / 14.2 / 22  18.0 / 15.9 / 26  25.8 / 26.8 / 30  30.2 / 28.2 / 33
+//    16 rows   14.8 / 17.7 / 26  24.7 / 18.0 / 26  26.5 / 20.8 / 29  37.2 / 34.4 / 33  46.3 / 37.1 / 35
+// The rule is on the wrong side between one and 5/4 workgroups a CU (N = 4608: 1 row 5.8 / 5.3, 16 rows 9.2 / 7.0), for
+// 16 rows between 8192 and 12288 (10240: 11.8 / 9.2), and on the longest sums and widest weights, where four tiles hold
+// more than the registers (14 of them spilled; 16 x 17408 x 17408 48.8 / 56.5).
 static hipError_t gemm_rows(const Product& c, hipStream_t stream) {
   const Layout L(c.N, c.K);
   const int per = (L.KS + ROW_WAVES - 1) / ROW_WAVES, waves = (L.KS + per - 1) / per, xt = (c.n + 15) / 16;
@@ -149,16 +157,17 @@ static hipError_t gemm_rows(const Product& c, hipStream_t stream) {
 // workgroups that take turns on a CU (a little longer while every CU has one), but no less than reading the weight at
 // 7 TB/s, longer by what the last turn leaves idle (32 x 34816 x 5120: 32.8 on 272 tiles of 32 x 128, 24.2 on 136 of
 // 64 x 256); a workgroup's start and end; and outputs (MB; a split writes and reads fp32 as well). The constants are
-// least squares over 120 calls from 17 x 80 x 64 to 2048 x 34816 x 5120, on which the choice is 2 % behind the best
-// kernel and split, 18 % at most. us, tiles of 256 x 256 / 256 x 160 / 128 x 256 / 64 x 256 / 64 x 128 / 32 x 128 /
-// 32 x 64:
+// least squares over 120 calls from 17 x 80 x 64 to 2048 x 34816 x 5120, of block kernels that have become 15 to 20 %
+// faster since (300 x 5120 x 6144 is priced 18.0 us and takes 14.5). On 128 calls of today's, 17 to 2048 rows, the
+// choice is 1.8 % behind the best kernel and split on average, 22 % at most (26 x 16937 x 4704: 18.2, 14.9 on 32 x 128
+// alone). us, tiles of 256 x 256 / 256 x 160 / 128 x 256 / 64 x 256 / 64 x 128 / 32 x 128 / 32 x 64:
 //   2048 x 34816 x 5120  281 / 295 / 326 / 425 / 491 / - / 1128
-//   2048 x 5120 x 6144   57 / 51 / 70 / 77 / 88 / - / 198
+//   2048 x 5120 x 6144   60 / 51 / 68 / 75 / 83 / 125 / 197
 //   1024 x 5120 x 5120   46 / 33 / 29 / 39 / 37 / - / 80
-//   64 x 34816 x 5120    45 / 37 / 35 / 32 / 39 / 41 / 46 (272 tiles of 64 x 128 on 256 CUs, 136 of 64 x 256)
-//   300 x 5120 x 6144    53 / 37 / 31 / 20 / 15 / 20 / 27
+//   64 x 34816 x 5120    46 / 38 / 36 / 30 / 35 / 41 / 47 (272 tiles of 64 x 128 on 256 CUs, 136 of 64 x 256)
+//   300 x 5120 x 6144    53 / 38 / 31 / 20 / 15.6 / 21 / 27
 //   687 x 1326 x 5056    - / - / - / - / 15.8 / 12.6 / -
-//   77 x 5001 x 6176     55 / 38 / 33 / 25 / 19 / 13.6 / 10.7
+//   77 x 5001 x 6176     56 / 38 / 34 / 25 / 19 / 14.3 / 11.4
 // Splits: 128 x 5120 x 17408 on 64 x 128, 48 us in one part, 31 in 2, 34 in 4; 40 x 100 x 17408 on 32 x 64, 16 in
 // one, 9 in 4.
 struct Cost {
@@ -216,8 +225,9 @@ static Choice choose(int n, int N, int K, size_t ws_bytes, long cus) {
 }
 
 // A call, or two: the weight rows whose tiles give every CU the same number, and the others by what suits them (two
-// launches: by 3 % at least). 2048 x 34816 x 5120 is 1088 tiles of 256 x 256, 4.25 a CU: 282 us, with the last 2048
-// weight rows in 256 blocks of 64 x 256 274 us; 1024 x 34816 x 5120 165 and 139 us.
+// launches: by 3 % at least). 2048 x 34816 x 5120 is 1088 tiles of 256 x 256, 4.25 a CU: 281 us, with the last 2048
+// weight rows in 256 blocks of 64 x 256 275 us (both in turn on one card, 40 calls in a row; one call by itself 279 and
+// 260); 1024 x 34816 x 5120 165 and 140 us.
 struct Plan {
   Choice first, rest;
   int cut;  // weight rows of the first; N if that is all

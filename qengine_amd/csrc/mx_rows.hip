@@ -60,15 +60,15 @@ __device__ __forceinline__ void store8(const float (&v)[8], uint8_t* q, uint8_t*
   if ((c & 3) == 0) s[c >> 2] = (uint8_t)code;
 }
 
-// silu(g) * u, g >= FAR. exp and the reciprocal are the instructions' (1 ulp each, 2^-23); the exponential's argument is
-// off by 2^-24 (its rounding) and 2^-26 (the constant's) of itself. In all (0.61 |g| + 4) 2^-23 of the value, 2^-17 at
-// the most, far below the code's 2^-4.
+// silu(g) * u, g >= FAR. exp and the reciprocal are the instructions' (1 ulp each, 2^-23); the exponential's argument
+// is off by 2^-24 (its rounding) and 2^-26 (the constant's) of itself. In all (0.61 |g| + 4) 2^-23 of the value, 2^-17
+// at the most, far below the code's 2^-4.
 constexpr float FAR = -64.f;
 __device__ __forceinline__ float swiglu(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g)) * u;
 }
-// The same below FAR, where 1 + e^-g is e^-g in fp32 and leaves its range from g = -88 on, while g e^g u need not: e^g as a
-// fraction in [1/2, 1) and an exponent that u takes first. Nothing below -300 has a code.
+// The same below FAR, where 1 + e^-g is e^-g in fp32 and leaves its range from g = -88 on, while g e^g u need not: e^g
+// as a fraction in [1/2, 1) and an exponent that u takes first. Below 2^-300 no u has a code.
 __device__ __forceinline__ float swiglu_far(float g, float u) {
   const float x = fmaxf(1.44269504f * g, -300.f), e = floorf(x) + 1.f;
   return g * ldexpf(__builtin_amdgcn_exp2f(x - e) * u, (int)e);

@@ -4,8 +4,9 @@
 // bytes of scales, both contiguous. In bf16 a lane holds 8 neighbouring values, a quad a block, and 16 lanes a row's
 // 256 bytes, so that one instruction covers 4 rows by two whole lines; in codes a lane has 16 bytes, a block of one
 // row. A quad turns one into the other: lane q's dword of row 4 i + l is dword q of lane i, a 4 x 4 transposition.
-// 34816 x 5120: 80 us there, 79 us back, 5.7 TB/s, more than a large copy reaches (4.9; with a block of 64 bytes a
-// lane, whose instructions touch 64 lines each, 130 us).
+// 34816 x 5120, four weights in turn: 81 us there, 79 us back (5.6 and 5.7 TB/s; a large copy reaches 4.8, but reads
+// as much as it writes), 173 us as a pair, where each begins behind the other's stores. With a block of 64 bytes a
+// lane, whose instructions touch 64 lines each, 130 us one way.
 #include <limits.h>
 
 #include <type_traits>
