@@ -103,7 +103,7 @@ def test_splits(native, kernel):
     rows, cols = TILES[kernel]
     n, N = rows + 5, cols + 13
     ran = set()
-    for b in (8, 12, 15, 20, 29, 33, 36, 37, 44, 61, 64, 68, 83, 96, 110, 128, 131, 134, 193, 261, 264, 266, 330, 544):
+    for b in (8, 12, 15, 20, 29, 33, 36, 37, 44, 61, 64, 68, 83, 97, 110, 128, 131, 134, 193, 261, 264, 266, 330, 544):
         K, g = 32 * b, C.gen(b)
         q, s = rows8(g, n, K)
         wq, wv = weights(native, g, N, K)
